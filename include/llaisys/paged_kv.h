@@ -62,6 +62,7 @@ LLAISYS_API const char *llaisysGetLastError(void);
 #define LLAISYS_KERNEL_GATES_TC 9         /* gated attention of chunks on tcgen05 tensor cores                    */
 #define LLAISYS_KERNEL_LATENT_TC 10       /* attention over pages of latents (mixers.h) on tcgen05 tensor cores   */
 #define LLAISYS_KERNEL_EXPANDED_TC 11     /* chunk attention over keys and values made from latents, tcgen05      */
+#define LLAISYS_KERNEL_EIGHT_BIT 12       /* attention over pages held in 8 bits                                  */
 /* Kernel of the calling thread's most recent attention call: any cache, or llaisysSelfAttention. */
 LLAISYS_API int llaisysLastAttentionKernel(void);
 
@@ -78,6 +79,25 @@ LLAISYS_API int llaisysPagedKVCreate(llaisysPagedKV_t *kv_out, llaisysDeviceType
                                      llaisysDataType_t dtype, size_t nlayer, size_t num_pages, size_t page_size,
                                      size_t nkvh, size_t head_dim, size_t max_seqs, size_t max_pages_per_seq);
 LLAISYS_API int llaisysPagedKVDestroy(llaisysPagedKV_t kv);
+
+/* A cache whose K and V are held in 8 bits, for activations of `dtype` (F32, F16 or BF16): the pool takes half (of F32: a quarter) of the
+ * memory, and of the bytes that attention reads. NVIDIA devices; page_size a multiple of 16, head_dim a multiple of 32 up to 256.
+ *   store LLAISYS_DTYPE_I8: codes are integers c, |c| <= M = 127; LLAISYS_DTYPE_F8: e4m3 numbers, |c| <= M = 448.
+ * 16 neighbouring token slots are a BLOCK; K and V of a block each have one f32 scale s per kv head, and a code is worth c * s. Rows that
+ * a call appends to a block (all in f32, products and quotients rounded once):
+ *     s' = max(s, max|x| / M, 2^-100)   over the rows' numbers x; s only where the first of them does not go to the block's slot 0
+ *     c  = round(x * (1 / s'))          to nearest, ties to even;   tokens in front of the rows, where s' > s:  c = round(c * (s * (1 / s')))
+ * so that a block filled token by token is rounded again only when its scale grows. A block that a NaN or an infinity is appended to
+ * gets the scale NaN, and attention of every query that reads the block is NaN, until its slot 0 is written again. Slots never written
+ * read as zero.
+ * The block manager, llaisysPagedKVAppend(Dev), Gather(Dev), llaisysPagedAttentionDecode(Dev), ...Prefill(Dev), ...DecodePartial(Dev) and
+ * llaisysPagedAttentionOptDev (mixers.h) take such a cache with rows, queries and outputs of `dtype`; every other call returns
+ * LLAISYS_E_UNSUPPORTED. The rows that one append call brings to a block must be neighbours in the call, in the order of their
+ * positions and without gaps (the host form checks this; the Dev form does not, and the block's content is undefined where it
+ * fails); rows with sequence -1 are skipped. The layout inside the pool is the library's own. */
+LLAISYS_API int llaisysPagedKVCreateQuantized(llaisysPagedKV_t *kv_out, llaisysDeviceType_t device_type, int device_id,
+                                              llaisysDataType_t dtype, llaisysDataType_t store, size_t nlayer, size_t num_pages,
+                                              size_t page_size, size_t nkvh, size_t head_dim, size_t max_seqs, size_t max_pages_per_seq);
 
 /* ---- block manager (host only; no device work) ---------------------------------------- */
 
@@ -203,6 +223,10 @@ LLAISYS_API int llaisysLseMerge(llaisysDeviceType_t device_type, int device_id, 
 LLAISYS_API int llaisysPagedKVAppendDev(llaisysPagedKV_t kv, size_t layer, const void *k_rows, const void *v_rows,
                                         const int32_t *seq_ids_dev, const int32_t *positions_dev, size_t n_rows,
                                         llaisysStream_t stream);
+/* Inverse of llaisysPagedKVAppendDev: token positions_dev[i] of sequence seq_ids_dev[i] -> row i of k_out, v_out [n_rows, nkvh, head_dim],
+ * in any order. Rows whose sequence or position does not exist are left as they were. */
+LLAISYS_API int llaisysPagedKVGatherDev(llaisysPagedKV_t kv, size_t layer, void *k_out, void *v_out, const int32_t *seq_ids_dev,
+                                        const int32_t *positions_dev, size_t n_rows, llaisysStream_t stream);
 /* The step before attention, fused: qkv is the packed q|k|v projection [n_rows, (nh + 2 nkvh) * head_dim] of the cache's
  * dtype, bias an optional row of the same width (NULL = none). q and k heads get the half-split rotary embedding of the
  * reference's rope operator (angle = position / theta^(2j/d), computed in float; reference: README.md rope section,
@@ -233,6 +257,40 @@ LLAISYS_API int llaisysPagedAttentionPrefillDev(llaisysPagedKV_t kv, size_t laye
                                                 const int32_t *kv_lens_dev, size_t n_seqs, size_t total_q,
                                                 size_t max_q_len, size_t max_kv_len, size_t nh, float scale,
                                                 llaisysStream_t stream);
+
+/* ---- index arrays of a step, made on the GPU ----------------------------------------------------- */
+/* From what every request holds and brings to what the calls of a step take, in one launch, nothing read back. Request i (row seq_ids_dev[i]
+ * of the block table; NULL: row i) holds held_dev[i] tokens and brings new_dev[i] (0: it sits the step out). With pages(t) = ceil(t / page_size):
+ *   q_starts_dev [n_seqs + 1]     sums of new in front of request i, the total at the end    (q_starts of the chunk calls)
+ *   kv_lens_dev [n_seqs]          held + new                                               (kv_lens of the attention calls)
+ *   page_starts_dev [n_seqs + 1]  sums of pages(held + new), likewise
+ *   row_seqs_dev, row_positions_dev [n_rows], row r of request i: its table row, and held + r - q_starts[i]    (of the append calls)
+ *   row_slots_dev [n_rows]        page * page_size + slot of that token, through the table as this call leaves it
+ *   block_table_dev [table_rows][table_stride]: entries [pages(held), pages(held + new)) of request i, requests in order, take
+ *                                 free_pages_dev[0], [1], ...; NULL free_pages_dev: the table is complete already and only read
+ *   status_dev [2]                pages taken, and LLAISYS_PLAN_ bits
+ * Any output may be NULL, and so may the table when neither slots nor growth are wanted. Rows behind the last request's, up to n_rows, are -1
+ * (such rows are skipped by appends to a cache held in 8 bits). A request may appear once.
+ * What cannot be done is left out and flagged, never written elsewhere: too few free pages take none at all (slots on missing pages are -1);
+ * rows behind n_rows are dropped (q_starts ends at n_rows); negative counts and sums over 2^31 - 1 count as nothing brought; a request whose row
+ * or last page lies outside the table gets no page and slots of -1 there. */
+#define LLAISYS_PLAN_NO_PAGES 1
+#define LLAISYS_PLAN_ROWS_DROPPED 2
+#define LLAISYS_PLAN_BAD_COUNT 4
+#define LLAISYS_PLAN_BAD_ROW 8
+struct LlaisysPagedPlan {
+    const int32_t *seq_ids_dev, *held_dev, *new_dev;
+    size_t n_seqs, page_size, n_rows;
+    const int32_t *free_pages_dev;
+    size_t n_free;
+    int32_t *block_table_dev;
+    size_t table_rows, table_stride;
+    int32_t *q_starts_dev, *kv_lens_dev, *page_starts_dev, *row_seqs_dev, *row_positions_dev;
+    int64_t *row_slots_dev;
+    int32_t *status_dev;
+};
+LLAISYS_API int llaisysPagedPlanDev(llaisysDeviceType_t device_type, int device_id, const struct LlaisysPagedPlan *args,
+                                    llaisysStream_t stream);
 
 /* ---- decode without any allocation ------------------------------------------------------------- */
 /* No counterpart in the reference. For callers that cannot let a library allocate device memory: a server that

@@ -88,6 +88,84 @@ int llaisysPagedKVCreate(llaisysPagedKV_t *kv_out, llaisysDeviceType_t device_ty
     });
 }
 
+int llaisysPagedKVCreateQuantized(llaisysPagedKV_t *kv_out, llaisysDeviceType_t device_type, int device_id, llaisysDataType_t dtype,
+                                  llaisysDataType_t store, size_t nlayer, size_t num_pages, size_t page_size, size_t nkvh, size_t head_dim,
+                                  size_t max_seqs, size_t max_pages_per_seq) {
+    return guarded([&] {
+        if (kv_out == nullptr) {
+            throw llaisys::kv::StatusError(LLAISYS_E_INVALID, "paged KV: kv_out is null");
+        }
+        *kv_out = nullptr;
+        if (store != LLAISYS_DTYPE_I8 && store != LLAISYS_DTYPE_F8) {
+            throw llaisys::kv::StatusError(LLAISYS_E_INVALID, "paged KV: 8-bit pages hold I8 or F8");
+        }
+        llaisys::kv::PagedKVConfig cfg;
+        cfg.device_type = device_type;
+        cfg.device_id = device_id;
+        cfg.dtype = dtype;
+        cfg.store = store;
+        cfg.nlayer = nlayer;
+        cfg.num_pages = num_pages;
+        cfg.page_size = page_size;
+        cfg.nkvh = nkvh;
+        cfg.head_dim = head_dim;
+        cfg.max_seqs = max_seqs;
+        cfg.max_pages_per_seq = max_pages_per_seq;
+        *kv_out = new LlaisysPagedKV(cfg);
+    });
+}
+
+int llaisysPagedPlanDev(llaisysDeviceType_t device_type, int device_id, const LlaisysPagedPlan *a, llaisysStream_t stream) {
+    return guarded([&] {
+        using llaisys::kv::StatusError;
+        constexpr size_t kMost = 0x7fffffff;
+        if (a == nullptr || (a->n_seqs != 0 && (a->held_dev == nullptr || a->new_dev == nullptr))) {
+            throw StatusError(LLAISYS_E_INVALID, "paged plan: null argument");
+        }
+        const size_t sizes[] = {a->n_seqs, a->n_rows, a->n_free, a->table_rows, a->table_stride};
+        for (size_t s : sizes) {
+            if (s >= kMost) {
+                throw StatusError(LLAISYS_E_INVALID, "paged plan: sizes must fit 32-bit indices");
+            }
+        }
+        if (a->page_size == 0 || a->page_size > kMost) {
+            throw StatusError(LLAISYS_E_INVALID, "paged plan: page_size must be positive");
+        }
+        if (a->block_table_dev == nullptr && (a->row_slots_dev != nullptr || a->free_pages_dev != nullptr)) {
+            throw StatusError(LLAISYS_E_INVALID, "paged plan: slots and growth need the block table");
+        }
+        if (device_type != LLAISYS_DEVICE_NVIDIA) {
+            throw StatusError(LLAISYS_E_UNSUPPORTED, "paged plan: NVIDIA devices only");
+        }
+#ifdef ENABLE_NVIDIA_API
+        llaisys::core::context().setDevice(device_type, device_id);
+        llaisys::kernels::PlanArgs p;
+        p.seq_ids = a->seq_ids_dev;
+        p.held = a->held_dev;
+        p.fresh = a->new_dev;
+        p.n_seqs = int32_t(a->n_seqs);
+        p.page_size = int32_t(a->page_size);
+        p.n_rows = int32_t(a->n_rows);
+        p.free_pages = a->free_pages_dev;
+        p.n_free = a->free_pages_dev ? int32_t(a->n_free) : 0;
+        p.table = a->block_table_dev;
+        p.table_rows = a->block_table_dev ? int32_t(a->table_rows) : 0;
+        p.table_stride = int32_t(a->table_stride);
+        p.q_starts = a->q_starts_dev;
+        p.kv_lens = a->kv_lens_dev;
+        p.page_starts = a->page_starts_dev;
+        p.row_seqs = a->row_seqs_dev;
+        p.row_positions = a->row_positions_dev;
+        p.row_slots = a->row_slots_dev;
+        p.status = a->status_dev;
+        llaisys::kernels::paged_plan(stream, p);
+#else
+        (void)device_id, (void)stream;
+        throw StatusError(LLAISYS_E_UNSUPPORTED, "this build has no NVIDIA backend");
+#endif
+    });
+}
+
 int llaisysPagedKVDestroy(llaisysPagedKV_t kv) {
     return guarded([&] { delete kv; });
 }
@@ -356,6 +434,11 @@ int llaisysPagedKVAppendDev(llaisysPagedKV_t kv, size_t layer, const void *k_row
                             llaisysStream_t stream) {
     KV_OR_FAIL(kv);
     return guarded([&] { kv->impl.appendDev(layer, k_rows, v_rows, seq_ids_dev, positions_dev, n_rows, stream); });
+}
+int llaisysPagedKVGatherDev(llaisysPagedKV_t kv, size_t layer, void *k_out, void *v_out, const int32_t *seq_ids_dev,
+                            const int32_t *positions_dev, size_t n_rows, llaisysStream_t stream) {
+    KV_OR_FAIL(kv);
+    return guarded([&] { kv->impl.gatherDev(layer, k_out, v_out, seq_ids_dev, positions_dev, n_rows, stream); });
 }
 int llaisysPagedKVRopeAppendDev(llaisysPagedKV_t kv, size_t layer, void *q_out, const void *qkv, const void *bias,
                                 const int32_t *seq_ids_dev, const int32_t *positions_dev, size_t n_rows, size_t nh,

@@ -253,6 +253,29 @@ int paged_gather(size_t elem_size, const KVView &kv, int32_t seq_row, int32_t n_
     return err;
 }
 
+int paged_gather_rows(size_t elem_size, const KVView &kv, int32_t table_rows, const int32_t *seq_ids, const int32_t *positions, int32_t n_rows,
+                      void *k_out, void *v_out) {
+    int err = 0;
+    const size_t head_row = size_t(kv.d) * elem_size;
+    auto *ko = static_cast<std::byte *>(k_out);
+    auto *vo = static_cast<std::byte *>(v_out);
+    const auto *kp = static_cast<const std::byte *>(kv.k_base);
+    const auto *vp = static_cast<const std::byte *>(kv.v_base);
+    for (int32_t r = 0; r < n_rows; ++r) {
+        const int64_t off = slot_offset_bytes(kv, elem_size, seq_ids[r] < table_rows ? seq_ids[r] : -1, positions[r], kv.table_stride, &err);
+        if (off < 0) {
+            continue;
+        }
+        for (int32_t h = 0; h < kv.nkvh; ++h) {
+            const int64_t src = off + int64_t(h) * kv.head_stride * int64_t(elem_size);
+            const size_t dst = (size_t(r) * kv.nkvh + h) * head_row;
+            std::memcpy(ko + dst, kp + src, head_row);
+            std::memcpy(vo + dst, vp + src, head_row);
+        }
+    }
+    return err;
+}
+
 int attention(llaisysDataType_t dtype, const KVView &kv, const AttnBatch &batch, const void *q, float scale,
               const AttnOut &out) {
     if (batch.total_q <= 0 || batch.nh <= 0) {

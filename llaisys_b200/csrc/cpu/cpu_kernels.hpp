@@ -16,6 +16,8 @@ void rearrange(size_t elem_size, size_t ndim, const size_t *shape, const ptrdiff
 // Returns the OR of the kErr* bits (kernels/device_utils.cuh uses the same values) for rows it had to skip.
 int paged_append(size_t elem_size, const kernels::KVView &kv, const void *k_rows, const void *v_rows,
                  const int32_t *seq_ids, const int32_t *positions, int32_t n_rows, int32_t max_blocks);
+int paged_gather_rows(size_t elem_size, const kernels::KVView &kv, int32_t table_rows, const int32_t *seq_ids, const int32_t *positions, int32_t n_rows,
+                      void *k_out, void *v_out);
 int paged_gather(size_t elem_size, const kernels::KVView &kv, int32_t seq_row, int32_t n_tokens, void *k_out,
                  void *v_out);
 // Bias + rotary embedding + append over a packed projection qkv [n_rows, (nh + 2 nkvh) * d] (see kernels.hpp, K1b).

@@ -53,6 +53,31 @@ struct KVView {
     int64_t tma_page0 = 0;
 };
 
+// A layer of a page pool held in 8 bits. A TILE is K and V of one block of 16 tokens and one kv head with their scales (quant_tile.cuh);
+// tiles lie [page][block of the page][kv head].
+struct QuantView {
+    unsigned char *base = nullptr;
+    int64_t page_bytes = 0;
+    int32_t tile_bytes = 0;
+    int32_t blocks_per_page = 1, num_pages = 0, nkvh = 0, d = 0;
+    const int32_t *block_table = nullptr; // [table_rows][table_stride]
+    int32_t table_rows = 0, table_stride = 0;
+    bool f8 = false; // codes are e4m3 numbers, not integers
+};
+
+// The arrays of a step from its requests' lengths (see llaisysPagedPlanDev).
+struct PlanArgs {
+    const int32_t *seq_ids = nullptr, *held = nullptr, *fresh = nullptr;
+    int32_t n_seqs = 0, page_size = 0, n_rows = 0;
+    const int32_t *free_pages = nullptr;
+    int32_t n_free = 0;
+    int32_t *table = nullptr;
+    int32_t table_rows = 0, table_stride = 0;
+    int32_t *q_starts = nullptr, *kv_lens = nullptr, *page_starts = nullptr, *row_seqs = nullptr, *row_positions = nullptr;
+    int64_t *row_slots = nullptr;
+    int32_t *status = nullptr;
+};
+
 // Which queries attend to which sequences. Arrays live on the executing device; a null array selects the
 // scalar that follows it (the legacy single-sequence operator has no arrays to pass).
 struct AttnBatch {

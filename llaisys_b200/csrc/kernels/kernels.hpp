@@ -191,6 +191,18 @@ void rotary_table(stream_t stream, float *table, const int32_t *positions, const
 void softcap_argmax(stream_t stream, float *logits, float cap, int64_t *idx_out, size_t rows, size_t n, void *scratch);
 
 // K5: tokens [0, n_tokens) of table row seq_row -> k_out, v_out [n_tokens, nkvh, d].
+// Rows (seq_ids[i], positions[i]) of a page pool, in any order; rows that do not exist are left as they were and flagged.
+void paged_gather_rows(stream_t stream, size_t elem_size, const KVView &kv, int32_t table_rows, const int32_t *seq_ids, const int32_t *positions,
+                       int32_t n_rows, void *k_out, void *v_out, int32_t *error_flag);
+// A pool held in 8 bits: append, rows read back (seq_ids null: sequence seq_row, positions 0, 1, ...), attention.
+void quant_append(stream_t stream, llaisysDataType_t dtype, const QuantView &kv, const void *k_rows, const void *v_rows,
+                  const int32_t *seq_ids, const int32_t *positions, int32_t n_rows, int32_t *error_flag);
+void quant_gather(stream_t stream, llaisysDataType_t dtype, const QuantView &kv, const int32_t *seq_ids, const int32_t *positions,
+                  int32_t seq_row, int32_t n_rows, void *k_out, void *v_out, int32_t *error_flag);
+void attention_quant(stream_t stream, llaisysDataType_t dtype, const QuantView &kv, const AttnBatch &batch, const void *q, float scale,
+                     const AttnOut &out, const AttnScratch &scratch);
+// The index arrays of a step.
+void paged_plan(stream_t stream, const PlanArgs &args);
 void paged_gather(stream_t stream, size_t elem_size, const KVView &kv, int32_t seq_row, int32_t n_tokens,
                   void *k_out, void *v_out, int32_t *error_flag);
 

@@ -145,6 +145,28 @@ __global__ void small_copies_kernel(CopyList l) {
     }
 }
 
+// The rows that an append of the same index arrays would write: one thread per 16-byte piece, as in the gather of a sequence below.
+__global__ void paged_gather_rows_kernel(const uint4 *__restrict__ k_pool, const uint4 *__restrict__ v_pool, uint4 *__restrict__ k_out,
+                                         uint4 *__restrict__ v_out, const int32_t *__restrict__ table, const int32_t *__restrict__ seq_ids,
+                                         const int32_t *__restrict__ positions, CopyGeom g, int32_t table_rows, int32_t n_rows,
+                                         int32_t *error_flag) {
+    const int32_t vecs_per_row = g.vecs_per_head_row * g.nkvh;
+    const int64_t total = int64_t(n_rows) * vecs_per_row;
+    const int64_t stride = int64_t(gridDim.x) * blockDim.x;
+    for (int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += stride) {
+        const int32_t row = int32_t(i / vecs_per_row), in_row = int32_t(i - int64_t(row) * vecs_per_row);
+        const int32_t kvh = in_row / g.vecs_per_head_row, vec = in_row - kvh * g.vecs_per_head_row;
+        const int32_t seq = seq_ids[row];
+        int32_t page, slot;
+        if (!resolve_slot(table, g, seq < table_rows ? seq : -1, positions[row], g.table_stride, error_flag, page, slot)) {
+            continue;
+        }
+        const int64_t at = (int64_t(page) * g.page_stride_b + int64_t(kvh) * g.head_stride_b + int64_t(slot) * g.token_stride_b) / 16 + vec;
+        k_out[i] = k_pool[at];
+        v_out[i] = v_pool[at];
+    }
+}
+
 __global__ void paged_gather_kernel(const uint4 *__restrict__ k_pool, const uint4 *__restrict__ v_pool,
                                     uint4 *__restrict__ k_out, uint4 *__restrict__ v_out,
                                     const int32_t *__restrict__ table, CopyGeom g, int32_t seq_row, int32_t n_tokens,
@@ -956,6 +978,21 @@ void small_copies(stream_t stream, const void *const *src, void *const *dst, con
     const int block = 256;
     small_copies_kernel<<<grid_for(int64_t(most), block), block, 0, static_cast<cudaStream_t>(stream)>>>(l);
     check_launch("small_copies");
+}
+
+void paged_gather_rows(stream_t stream, size_t elem_size, const KVView &kv, int32_t table_rows, const int32_t *seq_ids, const int32_t *positions,
+                       int32_t n_rows, void *k_out, void *v_out, int32_t *error_flag) {
+    const CopyGeom g = make_geom(kv, elem_size);
+    const int64_t total = int64_t(n_rows) * g.vecs_per_head_row * g.nkvh;
+    if (total <= 0) {
+        return;
+    }
+    CHECK_ARGUMENT(aligned16(k_out) && aligned16(v_out), "paged gather: rows must be 16-byte aligned");
+    const int64_t blocks = std::min<int64_t>((total + 255) / 256, 16384);
+    paged_gather_rows_kernel<<<unsigned(blocks), 256, 0, static_cast<cudaStream_t>(stream)>>>(
+        static_cast<const uint4 *>(kv.k_base), static_cast<const uint4 *>(kv.v_base), static_cast<uint4 *>(k_out), static_cast<uint4 *>(v_out),
+        kv.block_table, seq_ids, positions, g, table_rows, n_rows, error_flag);
+    check_launch("paged_gather_rows");
 }
 
 void paged_gather(stream_t stream, size_t elem_size, const KVView &kv, int32_t seq_row, int32_t n_tokens,

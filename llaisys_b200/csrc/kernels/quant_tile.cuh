@@ -1,0 +1,70 @@
+// A tile of a page pool held in 8 bits: K and V of 16 tokens of one kv head with their two scales, and the codes' arithmetic.
+//
+// The codes lie in the order in which mma.sync m16n8k16 wants its B operand, so that a lane of the attention kernel fetches what it multiplies
+// with 16-byte loads that follow one another over the lanes: no swizzle, no ldmatrix, no transposition of V. With lane = 4 g + t:
+//   K, scores = Q K^T (n = token, k = dim): column c of score tile j is token 4 (c / 2) + 2 j + c % 2, and the four k elements of a lane in step s
+//      are the neighbours 16 s + 4 t ..+3 (the query's fragments follow the same order). Word (s, j) of lane (g, t), the four codes of token
+//      4 (g / 2) + 2 j + g % 2, is word u = 2 s + j of the lane;
+//   V, output = P V (n = dim, k = token): a lane's scores of the two tiles are those of tokens 4 t ..+3, which makes them its A fragment of P
+//      as they are; word i of lane (g, t) holds the codes of those tokens for dim 8 i + g.
+// Word u of a lane lies at 16 (32 (u / 4) + lane) + 4 (u % 4); V follows K, and behind both lie the f32 scales of K and of V and 8 bytes of nothing.
+#pragma once
+
+#include "device_utils.cuh"
+
+#include <cuda_fp8.h>
+
+namespace llaisys::kernels {
+
+constexpr int kQuantTokens = 16;           // tokens of a block
+constexpr float kQuantFloor = 0x1p-100f;   // smallest scale an append writes
+
+__host__ __device__ __forceinline__ int quant_k_at(int token, int dim) {
+    const int u = 2 * (dim >> 4) + ((token >> 1) & 1), lane = 4 * (2 * (token >> 2) + (token & 1)) + ((dim >> 2) & 3);
+    return 16 * (32 * (u >> 2) + lane) + 4 * (u & 3) + (dim & 3);
+}
+__host__ __device__ __forceinline__ int quant_v_at(int token, int dim) { // from the first V code
+    const int u = dim >> 3, lane = 4 * (dim & 7) + (token >> 2);
+    return 16 * (32 * (u >> 2) + lane) + 4 * (u & 3) + (token & 3);
+}
+__host__ __device__ __forceinline__ int quant_scales_at(int d) { return 2 * kQuantTokens * d; }
+
+// Codes of a store: kF8 = e4m3, else integers.
+template <bool kF8>
+__device__ __forceinline__ unsigned char quant_code(float x) {
+    if constexpr (kF8) {
+        return __nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3);
+    } else {
+        return static_cast<unsigned char>(static_cast<signed char>(max(-127, min(127, __float2int_rn(x)))));
+    }
+}
+template <bool kF8>
+__device__ __forceinline__ float quant_worth(unsigned char c) {
+    if constexpr (kF8) {
+        return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3)));
+    } else {
+        return float(static_cast<signed char>(c));
+    }
+}
+
+// Where a token lives. False (and flagged): not in the pool.
+__device__ __forceinline__ bool quant_tile_of(const QuantView &kv, int seq, int block, int32_t *error_flag, unsigned char *&tiles) {
+    const int in_table = block / kv.blocks_per_page;
+    if (seq < 0 || seq >= kv.table_rows) {
+        atomicOr(error_flag, kErrBadSeq);
+        return false;
+    }
+    if (block < 0 || in_table >= kv.table_stride) {
+        atomicOr(error_flag, kErrBadPosition);
+        return false;
+    }
+    const int page = kv.block_table[int64_t(seq) * kv.table_stride + in_table];
+    if (page < 0 || page >= kv.num_pages) {
+        atomicOr(error_flag, kErrBadPage);
+        return false;
+    }
+    tiles = kv.base + int64_t(page) * kv.page_bytes + int64_t(block - in_table * kv.blocks_per_page) * kv.nkvh * kv.tile_bytes;
+    return true;
+}
+
+} // namespace llaisys::kernels

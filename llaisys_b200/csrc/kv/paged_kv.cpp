@@ -14,6 +14,7 @@
 #include <cstring>
 #include <limits>
 #include <sstream>
+#include <unordered_set>
 
 namespace llaisys::kv {
 
@@ -43,6 +44,8 @@ void setWindow(kernels::AttnBatch &b, const PagedKVConfig &cfg, const AttnOption
     b.fade_b = opt.fade_b;
 }
 constexpr size_t kMaxDecodeSeqs = 1024; // sequences per launch of the TMA decode kernel
+constexpr size_t kQuantBlock = 16;      // tokens of an 8-bit cache that share a scale
+size_t quantTileBytes(size_t d) { return 2 * kQuantBlock * d + 16; } // K, V and their scales of a block and head
 
 } // namespace
 
@@ -58,8 +61,16 @@ PagedKV::PagedKV(const PagedKVConfig &cfg) : _cfg(cfg) {
                LLAISYS_E_INVALID, "paged KV: sizes must fit 32-bit indices");
     _elem = utils::dsize(cfg.dtype);
     const size_t align = 16 / _elem;
+    if (quantized()) {
+        KV_REQUIRE(cfg.store == LLAISYS_DTYPE_I8 || cfg.store == LLAISYS_DTYPE_F8, LLAISYS_E_INVALID, "paged KV: 8-bit pages hold I8 or F8");
+        KV_REQUIRE(cfg.device_type != LLAISYS_DEVICE_CPU, LLAISYS_E_UNSUPPORTED, "paged KV: 8-bit pages on NVIDIA devices only");
+        KV_REQUIRE(cfg.layers.empty() && cfg.page_size % kQuantBlock == 0 && cfg.head_dim > 0 && cfg.head_dim % 32 == 0 && cfg.head_dim <= 256,
+                   LLAISYS_E_INVALID, "paged KV: 8-bit pages need a page size that is a multiple of 16 and a head_dim that is a multiple of 32 "
+                   "up to 256");
+        KV_REQUIRE(cfg.nkvh <= 65535, LLAISYS_E_INVALID, "paged KV: too many kv heads");
+    }
     if (_cfg.layers.empty()) {
-        KV_REQUIRE((cfg.head_dim * _elem) % 16 == 0, LLAISYS_E_INVALID,
+        KV_REQUIRE((cfg.head_dim * _elem) % 16 == 0 || quantized(), LLAISYS_E_INVALID,
                    "paged KV: a head row (head_dim * element size) must be a multiple of 16 bytes");
         _cfg.layers.assign(cfg.nlayer, KVLayerShape{cfg.nkvh, cfg.head_dim, cfg.head_dim});
     }
@@ -76,7 +87,8 @@ PagedKV::PagedKV(const PagedKVConfig &cfg) : _cfg(cfg) {
         l.v_row = shape.v_in_k ? 0 : (l.v_dim + align - 1) / align * align;
         l.page_elems = l.nkvh * cfg.page_size * (l.k_row + l.v_row);
         l.offset = pool_bytes;
-        l.bytes = cfg.num_pages * l.page_elems * _elem;
+        l.page_bytes = quantized() ? cfg.page_size / kQuantBlock * l.nkvh * quantTileBytes(l.k_dim) : l.page_elems * _elem;
+        l.bytes = cfg.num_pages * l.page_bytes;
         pool_bytes += (l.bytes + 255) / 256 * 256;
         max_kvh = std::max(max_kvh, l.nkvh);
         _layers.push_back(l);
@@ -104,7 +116,7 @@ PagedKV::PagedKV(const PagedKVConfig &cfg) : _cfg(cfg) {
         rt.synchronize();
         bool any_tma = false;
         for (Layer &l : _layers) {
-            if (_elem != 2 || l.k_dim != 128 || l.v_dim != 128 || l.v_row == 0 || cfg.page_size != 16) {
+            if (quantized() || _elem != 2 || l.k_dim != 128 || l.v_dim != 128 || l.v_row == 0 || cfg.page_size != 16) {
                 continue;
             }
             // one row of 128 elements per (page, K|V, kv-head, slot)
@@ -139,7 +151,7 @@ PagedKV::PagedKV(const PagedKVConfig &cfg) : _cfg(cfg) {
             }
         }
         size_t longest_v = 0; // of the layers that the gated tile kernel can serve
-        for (const Layer &l : _layers) {
+        for (const Layer &l : quantized() ? std::vector<Layer>() : _layers) {
             longest_v = std::max(longest_v, l.k_dim <= 128 && l.v_dim <= 128 ? l.v_dim : 0);
         }
         if (cfg.dtype == LLAISYS_DTYPE_BF16 && cfg.page_size == 16 && longest_v != 0) {
@@ -428,7 +440,7 @@ int32_t PagedKV::seqFork(int32_t parent, size_t n_tokens) {
         crow[cs.n_pages++] = dst;
         auto &rt = enter();
         for (const Layer &l : _layers) {
-            const size_t page_bytes = l.page_elems * _elem;
+            const size_t page_bytes = l.page_bytes;
             std::byte *base = _pool->memory() + l.offset;
             if (onDevice()) {
                 rt.api()->memcpy_async(base + size_t(dst) * page_bytes, base + size_t(src) * page_bytes, page_bytes,
@@ -500,6 +512,41 @@ int PagedKV::runGates(const kernels::KVView &v, const kernels::AttnBatch &b, con
     return used;
 #else
     (void)v, (void)b, (void)q, (void)scale, (void)gates, (void)o, (void)stream;
+    fail(LLAISYS_E_UNSUPPORTED, "this build has no NVIDIA backend");
+#endif
+}
+
+void PagedKV::requireWide(const char *what) const {
+    KV_REQUIRE(!quantized(), LLAISYS_E_UNSUPPORTED, "paged KV ", what, ": not for a cache held in 8 bits");
+}
+
+kernels::QuantView PagedKV::quantView(size_t layer) const {
+    const Layer &l = _layers[layer];
+    kernels::QuantView v;
+    v.base = reinterpret_cast<unsigned char *>(poolData(layer));
+    v.page_bytes = int64_t(l.page_bytes);
+    v.tile_bytes = int32_t(quantTileBytes(l.k_dim));
+    v.blocks_per_page = int32_t(_cfg.page_size / kQuantBlock);
+    v.num_pages = int32_t(_cfg.num_pages);
+    v.nkvh = int32_t(l.nkvh);
+    v.d = int32_t(l.k_dim);
+    v.block_table = blockTableData();
+    v.table_rows = int32_t(_cfg.max_seqs);
+    v.table_stride = int32_t(_cfg.max_pages_per_seq);
+    v.f8 = _cfg.store == LLAISYS_DTYPE_F8;
+    return v;
+}
+
+int PagedKV::runQuant(size_t layer, const kernels::AttnBatch &b, const void *q, float scale, const kernels::AttnOut &o, const AttnOptions &opt,
+                      llaisysStream_t stream) const {
+    KV_REQUIRE(opt.gates == nullptr && opt.fade_a == nullptr, LLAISYS_E_UNSUPPORTED,
+               "paged attention: gated weights and distance penalties not for a cache held in 8 bits");
+#ifdef ENABLE_NVIDIA_API
+    kernels::attention_quant(stream, _cfg.dtype, quantView(layer), b, q, scale, o, scratch());
+    noteAttentionKernel(LLAISYS_KERNEL_EIGHT_BIT);
+    return LLAISYS_KERNEL_EIGHT_BIT;
+#else
+    (void)layer, (void)b, (void)q, (void)scale, (void)o, (void)stream;
     fail(LLAISYS_E_UNSUPPORTED, "this build has no NVIDIA backend");
 #endif
 }
@@ -637,8 +684,41 @@ void PagedKV::appendDev(size_t layer, const void *k_rows, const void *v_rows, co
     }
 #ifdef ENABLE_NVIDIA_API
     enter();
+    if (quantized()) {
+        kernels::quant_append(stream, _cfg.dtype, quantView(layer), k_rows, v_rows, seq_ids_dev, positions_dev, int32_t(n_rows),
+                              reinterpret_cast<int32_t *>(_error_dev->memory()));
+        return;
+    }
     kernels::paged_append(stream, _elem, v, k_rows, v_rows, seq_ids_dev, positions_dev, int32_t(n_rows),
                           int32_t(_cfg.max_pages_per_seq), reinterpret_cast<int32_t *>(_error_dev->memory()));
+#else
+    (void)stream;
+    fail(LLAISYS_E_UNSUPPORTED, "this build has no NVIDIA backend");
+#endif
+}
+
+void PagedKV::gatherDev(size_t layer, void *k_out, void *v_out, const int32_t *seq_ids_dev, const int32_t *positions_dev, size_t n_rows,
+                        llaisysStream_t stream) {
+    checkLayer(layer);
+    KV_REQUIRE(n_rows <= kMaxInt32, LLAISYS_E_INVALID, "paged KV: too many rows");
+    if (n_rows == 0) {
+        return;
+    }
+    KV_REQUIRE(k_out && v_out && seq_ids_dev && positions_dev, LLAISYS_E_INVALID, "paged KV gather: null argument");
+    requireEqualRows(layer, "gather");
+    auto *error = reinterpret_cast<int32_t *>(_error_dev->memory());
+    if (!onDevice()) {
+        *error |= cpu::paged_gather_rows(_elem, view(layer), int32_t(_cfg.max_seqs), seq_ids_dev, positions_dev, int32_t(n_rows), k_out, v_out);
+        return;
+    }
+#ifdef ENABLE_NVIDIA_API
+    enter();
+    if (quantized()) {
+        kernels::quant_gather(stream, _cfg.dtype, quantView(layer), seq_ids_dev, positions_dev, 0, int32_t(n_rows), k_out, v_out, error);
+    } else {
+        kernels::paged_gather_rows(stream, _elem, view(layer), int32_t(_cfg.max_seqs), seq_ids_dev, positions_dev, int32_t(n_rows), k_out, v_out,
+                                   error);
+    }
 #else
     (void)stream;
     fail(LLAISYS_E_UNSUPPORTED, "this build has no NVIDIA backend");
@@ -648,6 +728,7 @@ void PagedKV::appendDev(size_t layer, const void *k_rows, const void *v_rows, co
 void PagedKV::ropeAppendDev(size_t layer, void *q_out, const void *qkv, const void *bias, const int32_t *seq_ids_dev,
                             const int32_t *positions_dev, size_t n_rows, size_t nh, float theta, llaisysStream_t stream) {
     checkLayer(layer);
+    requireWide("rope append");
     KV_REQUIRE(n_rows <= kMaxInt32 && nh > 0 && nh <= 4096, LLAISYS_E_INVALID, "paged KV rope append: bad sizes");
     KV_REQUIRE(_layers[layer].k_dim % 2 == 0, LLAISYS_E_INVALID, "paged KV rope append: head_dim must be even");
     if (n_rows == 0) {
@@ -675,6 +756,7 @@ void PagedKV::ropeAppendDev(size_t layer, void *q_out, const void *qkv, const vo
 
 void PagedKV::normAppendDev(size_t layer, const kernels::NormAppendArgs &args, llaisysStream_t stream) {
     checkLayer(layer);
+    requireWide("norm append");
     KV_REQUIRE(args.n_rows <= kMaxInt32 && args.nh > 0 && args.nh <= 4096, LLAISYS_E_INVALID, "paged KV norm append: bad sizes");
     if (args.n_rows == 0) {
         return;
@@ -783,6 +865,7 @@ void PagedKV::decodeStepDev(size_t layer, void *out, const void *q, const void *
                             const int32_t *seq_ids_dev, const int32_t *kv_lens_dev, size_t n_seqs, size_t max_kv_len,
                             size_t nh, float scale, llaisysStream_t stream) {
     checkLayer(layer);
+    requireWide("decode step");
     KV_REQUIRE(nh > 0 && nh % _layers[layer].nkvh == 0, LLAISYS_E_INVALID, "paged decode step: nh = ", nh,
                " is not a multiple of nkvh = ", _layers[layer].nkvh);
     KV_REQUIRE(n_seqs <= kMaxInt32 && max_kv_len <= _cfg.page_size * _cfg.max_pages_per_seq, LLAISYS_E_INVALID,
@@ -873,6 +956,8 @@ void PagedKV::launchDecode(size_t layer, void *out, float *part, const void *q, 
             }
             _last_kernel = LLAISYS_KERNEL_DECODE_TMA_FUSED;
             noteAttentionKernel(_last_kernel);
+        } else if (quantized()) {
+            _last_kernel = runQuant(layer, b, q_at, scale, o, opt, stream);
         } else if (opt.gates != nullptr) {
             _last_kernel = runGates(v, b, q_at, scale, *opt.gates, o, stream);
         } else {
@@ -927,7 +1012,8 @@ void PagedKV::prefillDev(size_t layer, void *out, const void *q, const int32_t *
     }
 #ifdef ENABLE_NVIDIA_API
     enter();
-    _last_kernel = opt.gates != nullptr ? runGates(v, b, q, scale, *opt.gates, o, stream)
+    _last_kernel = quantized()          ? runQuant(layer, b, q, scale, o, opt, stream)
+                   : opt.gates != nullptr ? runGates(v, b, q, scale, *opt.gates, o, stream)
                                         : run_attention_nvidia(stream, _cfg.dtype, v, b, q, scale, o, scratch());
 #else
     (void)stream;
@@ -949,6 +1035,15 @@ void PagedKV::append(size_t layer, const void *k_rows, const void *v_rows, const
         KV_REQUIRE(positions[i] >= 0 && size_t(positions[i]) < size_t(s.n_pages) * _cfg.page_size, LLAISYS_E_INVALID,
                    "paged KV append: row ", i, " position ", positions[i], " is beyond the ", s.n_pages,
                    " page(s) reserved for sequence ", seq_ids[i]);
+    }
+    if (quantized()) { // rows of a block: neighbours, ascending, once
+        std::unordered_set<uint64_t> seen;
+        auto block = [&](size_t i) { return (uint64_t(uint32_t(seq_ids[i])) << 32) | uint32_t(positions[i] / int32_t(kQuantBlock)); };
+        for (size_t i = 0; i < n_rows; ++i) {
+            const bool more = i > 0 && block(i) == block(i - 1);
+            KV_REQUIRE(more ? positions[i] == positions[i - 1] + 1 : seen.insert(block(i)).second, LLAISYS_E_INVALID, "paged KV append: row ", i,
+                       " (8-bit pages: the rows of a block of 16 tokens must be neighbours in the call, positions ascending by one)");
+        }
     }
     flush();
     if (!onDevice()) {
@@ -979,6 +1074,11 @@ void PagedKV::gather(size_t layer, int32_t seq, size_t n_tokens, void *k_out, vo
     }
 #ifdef ENABLE_NVIDIA_API
     auto &rt = enter();
+    if (quantized()) {
+        kernels::quant_gather(rt.stream(), _cfg.dtype, quantView(layer), nullptr, nullptr, seq, int32_t(n_tokens), k_out, v_out,
+                              reinterpret_cast<int32_t *>(_error_dev->memory()));
+        return;
+    }
     kernels::paged_gather(rt.stream(), _elem, v, seq, int32_t(n_tokens), k_out, v_out,
                           reinterpret_cast<int32_t *>(_error_dev->memory()));
 #else
@@ -1015,6 +1115,7 @@ void PagedKV::decodeStepHost(size_t layer, void *out_host, const void *q_host, c
                              const void *v_new_host, const int32_t *seq_ids, const int32_t *kv_lens, size_t n_seqs,
                              size_t nh, float scale) {
     checkLayer(layer);
+    requireWide("decode step");
     if (n_seqs == 0) {
         return;
     }

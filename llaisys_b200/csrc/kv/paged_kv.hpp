@@ -47,6 +47,8 @@ struct PagedKVConfig {
     size_t max_seqs = 0, max_pages_per_seq = 0;
     // one entry per layer when layers differ (or V rows are not as long as K rows): nkvh / head_dim above are ignored then
     std::vector<KVLayerShape> layers;
+    // I8 or F8: pages are held in 8 bits, rows and queries have `dtype`; INVALID: pages hold `dtype`
+    llaisysDataType_t store = LLAISYS_DTYPE_INVALID;
 };
 
 class PagedKV {
@@ -117,6 +119,9 @@ public:
     // qkv [n_rows, (nh + 2 nkvh) * d] (+ optional bias row) -> rotated q in q_out [n_rows, nh, d], rotated k and v appended
     void ropeAppendDev(size_t layer, void *q_out, const void *qkv, const void *bias, const int32_t *seq_ids_dev,
                        const int32_t *positions_dev, size_t n_rows, size_t nh, float theta, llaisysStream_t stream);
+    // rows of tokens (seq_ids_dev[i], positions_dev[i]) -> k_out, v_out [n_rows, nkvh, d]
+    void gatherDev(size_t layer, void *k_out, void *v_out, const int32_t *seq_ids_dev, const int32_t *positions_dev, size_t n_rows,
+                   llaisysStream_t stream);
     void decodeDev(size_t layer, void *out, float *part, const void *q, const int32_t *seq_ids_dev,
                    const int32_t *kv_lens_dev, size_t n_seqs, size_t max_kv_len, size_t nh, float scale,
                    llaisysStream_t stream, const AttnOptions &opt = {});
@@ -174,6 +179,11 @@ private:
     void checkLayer(size_t layer) const;
     void requireEqualRows(size_t layer, const char *what) const; // K and V rows of one length, unpadded
     void requireGates(const AttnOptions &opt) const;
+    bool quantized() const { return _cfg.store != LLAISYS_DTYPE_INVALID; }
+    void requireWide(const char *what) const; // pages that hold the activations' type
+    kernels::QuantView quantView(size_t layer) const;
+    int runQuant(size_t layer, const kernels::AttnBatch &b, const void *q, float scale, const kernels::AttnOut &o, const AttnOptions &opt,
+                 llaisysStream_t stream) const;
     // gated attention of one batch: the tile kernel where the shape allows, the generic one otherwise -> LLAISYS_KERNEL_*
     int runGates(const kernels::KVView &v, const kernels::AttnBatch &b, const void *q, float scale, const kernels::GateArgs &gates,
                  const kernels::AttnOut &o, llaisysStream_t stream) const;
@@ -196,7 +206,8 @@ private:
     // Geometry of one layer in the pool. Rows are padded to whole 16-byte pieces (k_row, v_row elements).
     struct Layer {
         size_t nkvh = 0, k_dim = 0, v_dim = 0, k_row = 0, v_row = 0; // v_row = 0: V rows lie in K rows
-        size_t page_elems = 0; // K and V of one page
+        size_t page_elems = 0; // K and V of one page (of pages that hold the activations' type)
+        size_t page_bytes = 0;
         size_t offset = 0, bytes = 0; // of the layer's pages in the pool
         // TMA view of the layer's pages (NVIDIA, 16-bit, K and V rows of 128, page 16 only)
         alignas(64) unsigned char tma_desc[128] = {};      // decode: box = K and V of a page

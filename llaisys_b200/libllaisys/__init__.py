@@ -297,6 +297,15 @@ class LlaisysGatedLinear(Structure):
                 ("scratch_segment_floats", c_size_t)]
 
 
+class LlaisysPagedPlan(Structure):
+    """struct LlaisysPagedPlan (include/llaisys/paged_kv.h)."""
+    _fields_ = [("seq_ids_dev", c_void_p), ("held_dev", c_void_p), ("new_dev", c_void_p), ("n_seqs", c_size_t), ("page_size", c_size_t),
+                ("n_rows", c_size_t), ("free_pages_dev", c_void_p), ("n_free", c_size_t), ("block_table_dev", c_void_p),
+                ("table_rows", c_size_t), ("table_stride", c_size_t), ("q_starts_dev", c_void_p), ("kv_lens_dev", c_void_p),
+                ("page_starts_dev", c_void_p), ("row_seqs_dev", c_void_p), ("row_positions_dev", c_void_p), ("row_slots_dev", c_void_p),
+                ("status_dev", c_void_p)]
+
+
 class LlaisysEngineEvent(Structure):
     """struct LlaisysEngineEvent (include/llaisys/serving.h)."""
     _fields_ = [("request", c_int64), ("token", c_int64), ("finished", c_int32), ("reserved", c_int32)]
@@ -376,6 +385,10 @@ PROTOTYPES: dict[str, tuple] = {
     "llaisysPagedKVSeqFork": (c_int, [_KV, c_int32, c_size_t, _I32P]),
     "llaisysPagedKVPageRefCount": (c_int, [_KV, c_int32]),
     "llaisysPagedKVNumCachedPages": (c_size_t, [_KV]),
+    "llaisysPagedKVCreateQuantized": (c_int, [POINTER(_KV), llaisysDeviceType_t, c_int, llaisysDataType_t, llaisysDataType_t, c_size_t, c_size_t,
+                                              c_size_t, c_size_t, c_size_t, c_size_t, c_size_t]),
+    "llaisysPagedKVGatherDev": (c_int, [_KV, c_size_t, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, llaisysStream_t]),
+    "llaisysPagedPlanDev": (c_int, [llaisysDeviceType_t, c_int, POINTER(LlaisysPagedPlan), llaisysStream_t]),
     "llaisysPagedKVRopeAppendDev": (c_int, [_KV, c_size_t, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t,
                                             c_size_t, c_float, llaisysStream_t]),
     "llaisysPagedAttentionDecodeDev": (c_int, [_KV, c_size_t, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t,

@@ -15,7 +15,7 @@ from typing import Sequence
 import numpy as np
 
 from .libllaisys import (LIB_LLAISYS, DataType, DeviceType, LlaisysExpandedAttention, LlaisysExperts, LlaisysGatedDelta, LlaisysGatedLinear,
-                         LlaisysGates, LlaisysLatentAppend, LlaisysMinGru, LlaisysNormAppend, LlaisysStateSpace, Status, llaisysPagedKV_t)
+                         LlaisysGates, LlaisysLatentAppend, LlaisysMinGru, LlaisysNormAppend, LlaisysPagedPlan, LlaisysStateSpace, Status, llaisysPagedKV_t)
 from .runtime import _addr
 
 _I32P = ctypes.POINTER(c_int32)
@@ -35,6 +35,7 @@ class Kernel(IntEnum):
     GATES_TC = 9
     LATENT_TC = 10
     EXPANDED_TC = 11
+    EIGHT_BIT = 12
 
 
 def last_attention_kernel() -> Kernel:
@@ -86,6 +87,24 @@ class PagedKVCache:
         _check(LIB_LLAISYS.llaisysPagedKVCreate(byref(handle), int(device), device_id, int(dtype), nlayer, num_pages,
                                                 page_size, nkvh, head_dim, max_seqs, self.max_pages_per_seq))
         self._kv = handle
+
+    @classmethod
+    def quantized(cls, num_pages: int, nkvh: int, head_dim: int, *, store: DataType = DataType.I8, page_size: int = 16, nlayer: int = 1,
+                  dtype: DataType = DataType.BF16, device: DeviceType = DeviceType.NVIDIA, device_id: int = 0, max_seqs: int = 256,
+                  max_pages_per_seq: int | None = None) -> "PagedKVCache":
+        """Cache whose K and V are held in 8 bits (store I8 or F8), a scale for each block of 16 tokens and kv head; rows, queries and outputs are
+        of `dtype` (see llaisysPagedKVCreateQuantized)."""
+        self = cls.__new__(cls)
+        self._kv = None
+        self.num_pages, self.nkvh, self.head_dim = num_pages, nkvh, head_dim
+        self.page_size, self.nlayer, self.dtype, self.store = page_size, nlayer, DataType(dtype), DataType(store)
+        self.device, self.device_id, self.max_seqs = DeviceType(device), device_id, max_seqs
+        self.max_pages_per_seq = max_pages_per_seq if max_pages_per_seq is not None else num_pages
+        handle = llaisysPagedKV_t()
+        _check(LIB_LLAISYS.llaisysPagedKVCreateQuantized(byref(handle), int(device), device_id, int(dtype), int(store), nlayer, num_pages,
+                                                         page_size, nkvh, head_dim, max_seqs, self.max_pages_per_seq))
+        self._kv = handle
+        return self
 
     def close(self) -> None:
         if self._kv is not None:
@@ -238,6 +257,11 @@ class PagedKVCache:
         _check(LIB_LLAISYS.llaisysPagedKVAppendDev(self._kv, layer, _addr(k_rows), _addr(v_rows), _addr(seq_ids_dev),
                                                    _addr(positions_dev), n_rows, stream))
 
+    def gather_dev(self, layer: int, k_out, v_out, seq_ids_dev, positions_dev, n_rows: int, stream) -> None:
+        """Inverse of append_dev: token positions[i] of sequence seq_ids[i] -> row i (device index arrays, explicit stream)."""
+        _check(LIB_LLAISYS.llaisysPagedKVGatherDev(self._kv, layer, _addr(k_out), _addr(v_out), _addr(seq_ids_dev),
+                                                   _addr(positions_dev), n_rows, stream))
+
     def rope_append_dev(self, layer: int, q_out, qkv, bias, seq_ids_dev, positions_dev, n_rows: int, nh: int,
                         theta: float, stream) -> None:
         """Bias + rotary embedding + append over a packed q|k|v projection (device index arrays, explicit stream)."""
@@ -355,6 +379,14 @@ class PagedKVCache:
         _check(LIB_LLAISYS.llaisysPagedAttentionGatesDev(
             self._kv, layer, _addr(out), _addr(q), _addr(seq_ids_dev), None if q_starts_dev is None else _addr(q_starts_dev),
             _addr(kv_lens_dev), n_seqs, total_q, max_q_len, max_kv_len, nh, scale, window, byref(gates), row_stride, stream))
+
+
+def paged_plan_dev(*, stream, device_id: int = 0, **fields) -> None:
+    """Index arrays of a step, slots and growth of the block table from the tokens that requests hold and bring, in one launch; fields of
+    LlaisysPagedPlan (include/llaisys/paged_kv.h), buffers may be tensors."""
+    numbers = {"n_seqs", "page_size", "n_rows", "n_free", "table_rows", "table_stride"}
+    args = LlaisysPagedPlan(**{k: (v if k in numbers or v is None else _addr(v)) for k, v in fields.items()})
+    _check(LIB_LLAISYS.llaisysPagedPlanDev(int(DeviceType.NVIDIA), device_id, byref(args), stream))
 
 
 def linear_row_dev(dtype: DataType, out, x, gain, eps: float, weight, n: int, k: int, form: int, *, stream, device_id: int = 0) -> None:

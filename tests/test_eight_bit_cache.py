@@ -1,0 +1,586 @@
+"""A paged cache held in 8 bits: append, rows read back and attention against the definitions, refusals, and a step planned on the GPU.
+
+The reference of the append is the definition in numpy, in f32 where the definition says so: rows read back have to equal it. Attention is
+compared with softmax in float64 over what the cache is worth.
+"""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+import llaisys_b200 as llaisys
+from llaisys_b200.libllaisys import LIB_LLAISYS, LlaisysPagedPlan, Status
+
+BLOCK = 16
+TORCH = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+NAMES = {"f32": llaisys.DataType.F32, "f16": llaisys.DataType.F16, "bf16": llaisys.DataType.BF16}
+STORES = {"i8": llaisys.DataType.I8, "f8": llaisys.DataType.F8}
+MOST = {"i8": np.float32(127), "f8": np.float32(448)}
+
+
+# ---- the definitions -----------------------------------------------------------------------------------------------------
+
+
+def code(x, store):
+    """Nearest code of f32 numbers that are divided by their scale, as the f32 number that it is."""
+    if store == "i8":
+        return np.clip(np.rint(x), -127, 127).astype(np.float32)
+    return torch.from_numpy(np.clip(x, -448, 448)).to(torch.float8_e4m3fn).float().numpy()
+
+
+class Definition:
+    """K (or V) of one sequence: codes [token, head, dim] and a scale per block and head."""
+
+    def __init__(self, nkvh, d, store):
+        self.store, self.nkvh, self.d = store, nkvh, d
+        self.codes = np.zeros((0, nkvh, d), np.float32)
+        self.scales = np.zeros((0, nkvh), np.float32)
+
+    def append(self, at, rows):  # rows f32 [n, head, dim] to tokens at, at + 1, ...
+        n = at + len(rows)
+        if n > len(self.codes):
+            self.codes = np.concatenate([self.codes, np.zeros((n - len(self.codes), self.nkvh, self.d), np.float32)])
+            blocks = -(-n // BLOCK)
+            self.scales = np.concatenate([self.scales, np.zeros((max(0, blocks - len(self.scales)), self.nkvh), np.float32)])
+        while len(rows):
+            b, slot = divmod(at, BLOCK)
+            part, rows = rows[:BLOCK - slot], rows[BLOCK - slot:]
+            for h in range(self.nkvh):
+                x = part[:, h]
+                old = self.scales[b, h] if slot else np.float32(0)
+                if not np.isfinite(x).all() or np.isnan(old):
+                    self.scales[b, h] = np.nan
+                    self.codes[at:at + len(part), h] = 0
+                    continue
+                new = np.maximum(np.maximum(old, np.abs(x).max() / MOST[self.store]), np.float32(2.0 ** -100))
+                inverse = np.float32(1) / new
+                if new > old and slot:
+                    front = self.codes[b * BLOCK:at, h]
+                    self.codes[b * BLOCK:at, h] = code(front * (old * inverse), self.store)
+                self.codes[at:at + len(part), h] = code(x * inverse, self.store)
+                self.scales[b, h] = new
+            at += len(part)
+
+    def worth(self):  # f32, products rounded once
+        return self.codes * np.repeat(self.scales, BLOCK, 0)[:len(self.codes), :, None]
+
+
+def attention_f64(q, k, v, held, scale, window=0, keep=0):
+    """q [n, nh, d], k / v [tokens, nkvh, d] float64; query t sits at position held + t. -> output, and for every (row, head) the error that a
+    weight or a score may bring: max |v| and max sum |q| |k|."""
+    n, nh, d = q.shape
+    group = nh // k.shape[1]
+    i, j = torch.arange(n)[:, None] + held, torch.arange(len(k))[None, :]
+    seen = j <= i
+    if window:
+        seen &= (i - j < window) | (j < keep)
+    k, v = k.repeat_interleave(group, 1), v.repeat_interleave(group, 1)
+    s = torch.einsum("thd,jhd->htj", q, k) * scale
+    s = s.masked_fill(~seen, -torch.inf)
+    p = torch.where(seen.any(-1)[None, :, None], torch.softmax(s, -1), 0.0)
+    big = (torch.einsum("thd,jhd->htj", q.abs(), k.abs()) * abs(scale)).masked_fill(~seen, 0).amax(-1).T
+    top = torch.where(seen[None], v.abs().amax(-1).T[:, None, :], 0).amax(-1).T
+    return torch.einsum("htj,jhd->thd", p, v), top, big
+
+
+def tolerance(want, top, big, dtype, tokens, d):
+    """Half a step of the output's type, and for the arithmetic in between: scores are f32 sums of d / 16 partial sums of exact products (each
+    addition off by 2^-23 of the sum of magnitudes, by cutting), the query is carried to 2^-22 and factors cost 4 roundings; a score off by e
+    moves the output by 2 e max |v|. Weights are rounded to 16 bits for 16-bit types (2^-11 relative, weights below 2^-28 of the largest to 2^-39)
+    and carried to 2^-21 for f32; sums over the tokens add 2^-23 per 16 of them."""
+    half = torch.finfo(TORCH[dtype]).eps / 2
+    score = (d / 16 + 8) * 2.0 ** -22 * big
+    weight = (2.0 ** -21 if dtype == "f32" else 2.0 ** -11 * 1.01) + (tokens / 16 + 16) * 2.0 ** -23
+    return half * want.abs() + ((2 * score + 2 * weight) * top)[..., None] + 1e-30
+
+
+# ---- calls ---------------------------------------------------------------------------------------------------------------
+
+
+def i32(values):
+    return torch.tensor(values, dtype=torch.int32, device="cuda")
+
+
+def stream():
+    return torch.cuda.current_stream().cuda_stream
+
+
+class Filled:
+    """A cache with its definition beside it: sequences in pages of a scattered order."""
+
+    def __init__(self, lens, nkvh, d, dtype, store, page=16, extra=0, seed=0):
+        self.rng, self.dtype, self.store, self.page, self.nkvh, self.d = np.random.default_rng(seed), dtype, store, page, nkvh, d
+        self.room = [-(-(n + extra) // page) for n in lens]
+        pages = sum(self.room) + 3
+        self.cache = llaisys.PagedKVCache.quantized(pages, nkvh, d, store=STORES[store], dtype=NAMES[dtype], page_size=page, max_seqs=len(lens) + 2,
+                                                    max_pages_per_seq=max(self.room + [1]))
+        order = self.rng.permutation(pages).tolist()
+        self.seqs = []
+        for n in self.room:
+            self.seqs.append(self.cache.add_seq())
+            self.cache.assign_pages(self.seqs[-1], [order.pop() for _ in range(n)])
+        self.k = [Definition(nkvh, d, store) for _ in lens]
+        self.v = [Definition(nkvh, d, store) for _ in lens]
+        self.append([(i, 0, n) for i, n in enumerate(lens) if n])
+
+    def rows(self, n):
+        x = self.rng.standard_normal((n, self.nkvh, self.d)) * np.exp(self.rng.uniform(-2, 2, (n, 1, 1)))
+        return torch.from_numpy(x).to(TORCH[self.dtype])
+
+    def append(self, parts, k=None, v=None):
+        """parts: (sequence, first position, count), one call."""
+        if not parts:
+            return
+        n = sum(c for _, _, c in parts)
+        k = self.rows(n) if k is None else k
+        v = self.rows(n) if v is None else v
+        seq = [self.seqs[i] for i, _, c in parts for _ in range(c)]
+        pos = [at + r for _, at, c in parts for r in range(c)]
+        self.cache.flush()
+        self.cache.append_dev(0, k.cuda(), v.cuda(), i32(seq), i32(pos), n, stream())
+        at = 0
+        for i, first, c in parts:
+            self.k[i].append(first, k[at:at + c].float().numpy())
+            self.v[i].append(first, v[at:at + c].float().numpy())
+            at += c
+
+    def check_rows(self):
+        """Every row read back equals the definition's."""
+        for i, seq in enumerate(self.seqs):
+            n = len(self.k[i].codes)
+            if n == 0:
+                continue
+            got = [torch.full((n, self.nkvh, self.d), 7.0, dtype=TORCH[self.dtype], device="cuda") for _ in range(2)]
+            self.cache.gather_dev(0, *got, i32([seq] * n), i32(range(n)), n, stream())
+            for g, want in zip(got, (self.k[i], self.v[i])):
+                w = torch.from_numpy(want.worth()).to(TORCH[self.dtype])
+                assert torch.equal(torch.isnan(g.cpu()), torch.isnan(w))
+                assert torch.equal(torch.nan_to_num(g.cpu().float()), torch.nan_to_num(w.float()))
+
+    def check_attention(self, parts, nh, window=0, keep=0, factor=None, stride=0, chunks=False, order=None):
+        """parts: (sequence, queries): the last tokens of each. Compares the call with the definition."""
+        group_rows = [n for _, n in parts]
+        total = sum(group_rows)
+        q = torch.randn(total + 2, nh, self.d, generator=torch.Generator().manual_seed(5)).to(TORCH[self.dtype])
+        width = stride or nh * self.d
+        out = torch.full((total + 2, width), 9.0, dtype=TORCH[self.dtype], device="cuda")
+        starts = np.concatenate([[0], np.cumsum(group_rows)])
+        lens = [len(self.k[i].codes) for i, _ in parts]
+        qd, ids, kv = q.cuda(), i32([self.seqs[i] for i, _ in parts]), i32(lens)
+        scale = self.d ** -0.5
+        kw = dict(n_seqs=len(parts), total_q=total, max_q_len=max(group_rows), max_kv_len=max(lens), nh=nh, scale=scale, stream=stream())
+        f = None if factor is None else factor.cuda()
+        self.cache.attention_dev(0, out, qd, ids, i32(starts) if chunks else None, kv, window=window, keep_first=keep, row_scale=f, row_stride=stride,
+                                 **kw)
+        got = out.cpu()
+        assert (got[total:] == 9).all() and (got[:, nh * self.d:] == 9).all()  # rows behind the last sequence, and between rows
+        got = got[:total, :nh * self.d].view(total, nh, self.d).double()
+        for (i, n), at in zip(parts, starts):
+            k, v = (torch.from_numpy(x.worth()).double() for x in (self.k[i], self.v[i]))
+            qs = q[at:at + n].double()
+            want, top, big = attention_f64(qs, k, v, len(k) - n, scale, window, keep)
+            tol = tolerance(want, top, big, self.dtype, len(k), self.d)
+            if factor is not None:
+                want, tol = want * factor[at:at + n].double()[..., None], tol * factor[at:at + n].double().abs()[..., None]
+            nan = torch.isnan(want)
+            assert torch.equal(nan, torch.isnan(got[at:at + n]))
+            worst = ((got[at:at + n] - want).abs() / tol)[~nan]
+            assert worst.numel() == 0 or worst.max() <= 1, (i, float(worst.max()))
+
+
+# ---- append --------------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("store", ["i8", "f8"])
+@pytest.mark.parametrize("dtype,nkvh,d,page", [("bf16", 2, 128, 16), ("f16", 3, 64, 32), ("f32", 1, 96, 16), ("bf16", 5, 256, 64), ("f32", 2, 32, 48)])
+def test_append_whole_and_in_pieces(cuda_device, store, dtype, nkvh, d, page):
+    f = Filled([1, 15, 16, 17, 0, 40, 130], nkvh, d, dtype, store, page, extra=60)
+    f.check_rows()
+    # pieces that begin inside blocks, one token at a time, and over several blocks; then tokens written again
+    f.append([(0, 1, 1), (1, 15, 20), (3, 17, 1), (4, 0, 5), (5, 40, 8)])
+    f.append([(0, 2, 1), (4, 5, 1), (5, 48, 1), (6, 130, 33)])
+    f.append([(6, 100, 3), (5, 0, 2), (3, 9, 4)])
+    f.check_rows()
+    f.cache.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("store", ["i8", "f8"])
+def test_append_token_by_token(cuda_device, store):
+    f = Filled([0, 3], 2, 64, "bf16", store, 16, extra=40)
+    for t in range(37):
+        f.append([(1, 3 + t, 1), (0, t, 1)])
+    f.check_rows()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("store", ["i8", "f8"])
+def test_append_zeros_extremes_and_what_is_not_finite(cuda_device, store):
+    f = Filled([0, 0, 0, 0], 2, 32, "f32", store, 16, extra=48)
+    zero = torch.zeros(20, 2, 32)
+    f.append([(0, 0, 20)], zero, zero)
+    f.append([(0, 20, 2)], torch.full((2, 2, 32), 1e-38), torch.full((2, 2, 32), 3e38))
+    rows = f.rows(20)
+    rows[3, 0, 5], rows[18, 1, 7] = torch.nan, -torch.inf
+    f.append([(1, 0, 20)], rows, f.rows(20))
+    f.append([(1, 20, 4)])   # behind a block that is lost
+    f.append([(1, 0, 16)])   # written again from its first slot: sound again
+    f.append([(2, 0, 5)])
+    f.append([(2, 5, 2)], torch.full((2, 2, 32), torch.nan), f.rows(2))
+    f.check_rows()
+
+
+@pytest.mark.gpu
+def test_append_skips_rows_without_sequence_and_flags_bad_ones(cuda_device):
+    f = Filled([20, 20], 2, 64, "bf16", "i8", 16, extra=12)
+    k = f.rows(6)
+    f.cache.append_dev(0, k.cuda(), k.cuda(), i32([-1, f.seqs[0], f.seqs[0], -1, -1, -1]), i32([-1, 20, 21, -1, 5, 0]), 6, stream())
+    f.k[0].append(20, k[1:3].float().numpy())
+    f.v[0].append(20, k[1:3].float().numpy())
+    f.cache.check()
+    f.check_rows()
+    for seq, pos in ((99, 0), (-2, 0), (0, -1), (0, 1 << 20)):
+        f.cache.append_dev(0, k.cuda(), k.cuda(), i32([seq]), i32([pos]), 1, stream())
+        with pytest.raises(llaisys.LlaisysError) as e:
+            f.cache.check()
+        assert e.value.status == Status.KERNEL
+        out = torch.full((1, 2, 64), 7.0, dtype=torch.bfloat16, device="cuda")
+        f.cache.gather_dev(0, out, out, i32([seq]), i32([pos]), 1, stream())
+        assert (out == 7).all()
+        with pytest.raises(llaisys.LlaisysError):
+            f.cache.check()
+    f.check_rows()
+
+
+@pytest.mark.gpu
+def test_host_forms_fork_and_prefix(cuda_device):
+    f = Filled([37, 5], 2, 64, "f16", "i8", 16, extra=20)
+    k, v = f.rows(4), f.rows(4)
+    kd, vd = k.cuda(), v.cuda()
+    f.cache.append(0, kd, vd, [f.seqs[0]] * 3 + [f.seqs[1]], [37, 38, 39, 5])
+    for i, part in ((0, slice(0, 3)), (1, slice(3, 4))):
+        f.k[i].append((37, 5)[i], k[part].float().numpy())
+        f.v[i].append((37, 5)[i], v[part].float().numpy())
+    out = [torch.empty(40, 2, 64, dtype=torch.float16, device="cuda") for _ in range(2)]
+    f.cache.gather(0, f.seqs[0], 40, *out)
+    torch.cuda.synchronize()
+    assert torch.equal(out[0].cpu().float(), torch.from_numpy(f.k[0].worth()).half().float())
+    child = f.cache.fork(f.seqs[0], 39)  # the last page is copied, scales and all
+    again = [torch.empty(39, 2, 64, dtype=torch.float16, device="cuda") for _ in range(2)]
+    f.cache.gather(0, child, 39, *again)
+    torch.cuda.synchronize()
+    assert torch.equal(again[0], out[0][:39]) and torch.equal(again[1], out[1][:39])
+    for seqs, pos in (([0, 0], [41, 40]), ([0, 1, 0], [41, 6, 42]), ([0, 0], [41, 41])):
+        with pytest.raises(llaisys.LlaisysError) as e:
+            f.cache.append(0, kd, vd, seqs, pos)
+        assert e.value.status == Status.INVALID
+    # decode, chunk and partial results through the host forms
+    q = torch.randn(2, 4, 64, dtype=torch.float16, device="cuda")
+    o, part = torch.empty_like(q), torch.empty(2, 4, 66, device="cuda")
+    f.cache.decode(0, o, q, f.seqs, [40, 6], 4, 0.125)
+    f.cache.decode_partial(0, part, q, f.seqs, [40, 6], 4, 0.125)
+    torch.cuda.synchronize()
+    assert torch.allclose(part[..., :64], o.float(), rtol=2.0 ** -10, atol=1e-6)
+    for i, n in enumerate((40, 6)):
+        ks = torch.from_numpy(f.k[i].worth()).double().repeat_interleave(2, 1)
+        s = torch.einsum("hd,jhd->hj", q[i].cpu().double(), ks) * 0.125
+        assert torch.allclose(part[i, :, 64].cpu().double(), s.amax(-1), rtol=1e-4, atol=1e-4)
+        assert torch.allclose(part[i, :, 65].cpu().double(), (s - s.amax(-1, keepdim=True)).exp().sum(-1), rtol=1e-3)
+
+
+# ---- attention -----------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("store", ["i8", "f8"])
+@pytest.mark.parametrize("dtype,nh,nkvh,d,page", [("bf16", 12, 2, 128, 16), ("f16", 8, 8, 64, 32), ("f32", 6, 3, 96, 16), ("bf16", 40, 2, 256, 64),
+                                                  ("f32", 4, 1, 128, 16), ("f16", 32, 1, 32, 48)])
+def test_decode(cuda_device, store, dtype, nh, nkvh, d, page):
+    f = Filled([1, 2, 15, 16, 17, 100, 333, 2050], nkvh, d, dtype, store, page)
+    f.check_attention([(i, 1) for i in (3, 0, 7, 1, 2, 6, 4, 5)], nh)
+    f.cache.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("store", ["i8", "f8"])
+@pytest.mark.parametrize("dtype,nh,nkvh,d,page", [("bf16", 12, 2, 128, 16), ("f16", 8, 2, 64, 32), ("f32", 6, 3, 96, 16), ("bf16", 17, 1, 128, 16),
+                                                  ("f32", 4, 4, 256, 64), ("f16", 32, 8, 128, 16)])
+def test_chunks(cuda_device, store, dtype, nh, nkvh, d, page):
+    f = Filled([1, 5, 16, 70, 200, 513, 1029], nkvh, d, dtype, store, page)
+    f.check_attention([(6, 300), (0, 1), (5, 17), (1, 5), (2, 2), (3, 33), (4, 200)], nh, chunks=True)
+    f.check_attention([(6, 1), (4, 1)], nh, chunks=True)
+    f.cache.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("window,keep", [(1, 0), (7, 3), (16, 16), (100, 20), (5000, 4), (33, 100)])
+@pytest.mark.parametrize("dtype,store,d", [("bf16", "i8", 128), ("f32", "f8", 64), ("f16", "f8", 128)])
+def test_windows_factors_and_strides(cuda_device, window, keep, dtype, store, d):
+    f = Filled([1, 40, 130, 777], 2, d, dtype, store)
+    factor = torch.randn(400, 8, generator=torch.Generator().manual_seed(3))
+    f.check_attention([(3, 1), (1, 1), (0, 1), (2, 1)], 8, window=window, keep=keep, factor=factor[:4], stride=8 * d + 8)
+    f.check_attention([(3, 260), (0, 1), (2, 100), (1, 39)], 8, window=window, keep=keep, factor=factor, stride=8 * d + 8, chunks=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_rows_that_see_nothing_and_lost_blocks(cuda_device, dtype):
+    f = Filled([40, 300], 2, 128, dtype, "i8")
+    q = torch.randn(3, 4, 128, device="cuda").to(TORCH[dtype])
+    out = torch.full_like(q, 9.0)
+    f.cache.decode_dev(0, out, q, i32([f.seqs[0], f.seqs[1], f.seqs[0]]), i32([40, 0, 0]), 3, 300, 4, 0.1, stream())
+    assert (out[1:] == 0).all() and not (out[0] == 0).all()
+    # more queries than tokens: the first ones see nothing
+    out.fill_(9.0)
+    f.cache.prefill_dev(0, out, q, i32([f.seqs[0]]), i32([0, 3]), i32([2]), 1, 3, 3, 2, 4, 0.1, stream())
+    assert (out[0] == 0).all() and not (out[1] == 0).all()
+    # a NaN in a block: queries that read the block are NaN, the others are not
+    bad = f.rows(1)
+    bad[0, 1, 5] = torch.nan
+    f.append([(1, 200, 1)], bad, f.rows(1))
+    f.check_attention([(1, 1)], 4)
+    f.check_attention([(1, 1)], 4, window=80)
+    f.check_attention([(1, 1)], 4, window=80, keep=16)
+
+
+@pytest.mark.gpu
+def test_one_long_sequence(cuda_device):
+    f = Filled([70001], 1, 64, "bf16", "i8")
+    f.check_attention([(0, 1)], 8)
+    f.check_attention([(0, 9)], 8, chunks=True)
+
+
+@pytest.mark.gpu
+def test_values_of_very_different_size(cuda_device):
+    """Blocks whose scales are far apart, and queries far from one."""
+    f = Filled([0], 2, 64, "f32", "i8", extra=200)
+    k, v = f.rows(180), f.rows(180)
+    v *= torch.exp2(torch.linspace(-60, 40, 180))[:, None, None]
+    k *= torch.exp2(torch.linspace(-90, -3, 180))[:, None, None]
+    f.append([(0, 0, 180)], k, v)
+    f.check_rows()
+    f.check_attention([(0, 1)], 4)
+    f.check_attention([(0, 60)], 4, chunks=True)
+
+
+# ---- a step, planned and run ----------------------------------------------------------------------------------------------
+
+
+def plan_reference(ids, held, new, page, rows, free, table):
+    table, q, p, at = table.copy(), [0], [0], 0
+    seqs, pos, slots = [], [], []
+    for i, h, n in zip(ids, held, new):
+        for e in range(-(-h // page), -(-(h + n) // page)):
+            table[i, e] = free[at]
+            at += 1
+        for t in range(h, h + n):
+            seqs.append(i)
+            pos.append(t)
+            slots.append(int(table[i, t // page]) * page + t % page)
+        q.append(q[-1] + n)
+        p.append(p[-1] + -(-(h + n) // page))
+    pad = [-1] * (rows - len(seqs))
+    return dict(q_starts=q, kv_lens=[h + n for h, n in zip(held, new)], page_starts=p, row_seqs=seqs + pad, row_positions=pos + pad,
+                row_slots=slots + pad, status=[at, 0]), table
+
+
+def run_plan(ids, held, new, page, rows, free, table, null_ids=False, skip=()):
+    n = len(held)
+    out = dict(q_starts=torch.full((n + 1,), -7, dtype=torch.int32, device="cuda"), kv_lens=torch.full((n,), -7, dtype=torch.int32, device="cuda"),
+               page_starts=torch.full((n + 1,), -7, dtype=torch.int32, device="cuda"), row_seqs=torch.full((rows,), -7, dtype=torch.int32, device="cuda"),
+               row_positions=torch.full((rows,), -7, dtype=torch.int32, device="cuda"),
+               row_slots=torch.full((rows,), -7, dtype=torch.int64, device="cuda"), status=torch.full((2,), -7, dtype=torch.int32, device="cuda"))
+    t = torch.from_numpy(table).cuda() if table is not None else None
+    f = i32(free) if free is not None else None
+    hd, nd, idd = i32(held), i32(new), None if null_ids else i32(ids)
+    llaisys.paged_plan_dev(stream=stream(), seq_ids_dev=idd, held_dev=hd, new_dev=nd, n_seqs=n, page_size=page, n_rows=rows, free_pages_dev=f,
+                           n_free=0 if free is None else len(free), block_table_dev=t, table_rows=0 if t is None else t.shape[0],
+                           table_stride=0 if t is None else t.shape[1], **{f"{k}_dev": None if k in skip else v for k, v in out.items()})
+    return {k: v.cpu().numpy() for k, v in out.items()}, None if t is None else t.cpu().numpy()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,low,high,short,long,page", [(1, 0, 0, 1, 1, 16), (1, 5, 5, 0, 0, 16), (7, 0, 40, 0, 3, 16), (64, 1, 4096, 1, 1, 16),
+                                                        (333, 0, 900, 0, 200, 32), (1024, 0, 50, 1, 2, 1), (2500, 0, 300, 0, 60, 48),
+                                                        (3, 0, 100, 20000, 30000, 16), (40000, 0, 20, 0, 2, 16)])
+def test_plan(cuda_device, n, low, high, short, long, page):
+    rng = np.random.default_rng(n)
+    held, new = rng.integers(low, high + 1, n), rng.integers(short, long + 1, n)
+    stride = max(1, int((-(-(held + new) // page)).max()))
+    ids = rng.permutation(n + 3)[:n]
+    table = rng.integers(0, 9999, (n + 3, stride)).astype(np.int32)
+    grown = int((-(-(held + new) // page) + -held // page).sum())
+    free = rng.permutation(grown + 5).astype(np.int32)
+    rows = int(new.sum()) + 70
+    got, t = run_plan(ids, held, new, page, rows, free, table)
+    want, w = plan_reference(ids.tolist(), held.tolist(), new.tolist(), page, rows, free, table)
+    for key, value in want.items():
+        assert np.array_equal(got[key], value), key
+    assert np.array_equal(t, w)
+
+
+@pytest.mark.gpu
+def test_plan_what_cannot_be_done(cuda_device):
+    table = np.arange(40, dtype=np.int32).reshape(4, 10)
+    # too few pages: none is taken, rows on pages that are there have slots
+    got, t = run_plan([0, 1], [10, 16], [10, 20], 16, 40, [90, 91], table)
+    assert np.array_equal(t, table) and got["status"].tolist() == [0, 1]
+    assert got["row_slots"][:10].tolist() == [0 * 16 + 10 + i for i in range(6)] + [-1] * 4 and (got["row_slots"][10:] == -1).all()
+    assert got["q_starts"].tolist() == [0, 10, 30] and got["kv_lens"].tolist() == [20, 36]
+    # rows that do not fit
+    got, t = run_plan([0, 1, 2], [0, 0, 0], [5, 6, 7], 16, 8, None, table)
+    assert got["q_starts"].tolist() == [0, 5, 8, 8] and got["status"].tolist() == [0, 2] and got["row_positions"].tolist() == [0, 1, 2, 3, 4, 0, 1, 2]
+    # counts that are none, rows outside the table, requests longer than their row
+    got, t = run_plan([0, 1, 7, 3], [-1, 2 ** 31 - 2, 3, 150], [4, 5, 2, 20], 16, 30, [50, 51, 52], table)
+    assert got["status"].tolist() == [0, 4 | 8] and got["q_starts"].tolist() == [0, 0, 0, 2, 22]
+    assert got["row_slots"][:2].tolist() == [-1, -1] and got["row_slots"][2:12].tolist() == [39 * 16 + 6 + i for i in range(10)]
+    assert (got["row_slots"][12:] == -1).all() and np.array_equal(t, table)
+    # nobody
+    got, t = run_plan([], [], [], 16, 3, [1], table)
+    assert got["q_starts"].tolist() == [0] and got["row_seqs"].tolist() == [-1] * 3 and got["status"].tolist() == [0, 0]
+    # no table, no ids, outputs left out
+    got, _ = run_plan(None, [4, 0], [1, 2], 16, 4, None, None, null_ids=True, skip=("row_slots", "page_starts", "status"))
+    assert got["row_seqs"].tolist() == [0, 1, 1, -1] and got["row_positions"].tolist() == [4, 0, 1, -1] and (got["row_slots"] == -7).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,store", [("bf16", "i8"), ("f32", "f8")])
+def test_steps_planned_on_the_gpu_and_replayed(cuda_device, dtype, store):
+    """Plan, append and attention of a few steps, nothing read back in between; the last form captured once and replayed with other lengths."""
+    n, nkvh, nh, d, most = 5, 2, 8, 64, 64
+    f = Filled([0] * n, nkvh, d, dtype, store, extra=160)
+    f.cache.flush()
+    held = np.array([0, 0, 0, 0, 0])
+    ids, q_starts, kv = i32(f.seqs), torch.empty(n + 1, dtype=torch.int32, device="cuda"), torch.empty(n, dtype=torch.int32, device="cuda")
+    seqs, pos = (torch.empty(most, dtype=torch.int32, device="cuda") for _ in range(2))
+    hd, nd = i32(held), i32(held)
+    k, v = (torch.zeros(most, nkvh, d, dtype=TORCH[dtype], device="cuda") for _ in range(2))
+    q, out = (torch.zeros(most, nh, d, dtype=TORCH[dtype], device="cuda") for _ in range(2))
+
+    def step():
+        llaisys.paged_plan_dev(stream=stream(), seq_ids_dev=ids, held_dev=hd, new_dev=nd, n_seqs=n, page_size=16, n_rows=most, q_starts_dev=q_starts,
+                               kv_lens_dev=kv, row_seqs_dev=seqs, row_positions_dev=pos)
+        f.cache.append_dev(0, k, v, seqs, pos, most, stream())
+        f.cache.attention_dev(0, out, q, ids, q_starts, kv, n_seqs=n, total_q=most, max_q_len=most, max_kv_len=160, nh=nh, scale=d ** -0.5,
+                              stream=stream())
+
+    graph = None
+    for turn, new in enumerate(([3, 20, 1, 0, 33], [1, 1, 1, 1, 1], [0, 17, 30, 5, 1], [1, 1, 0, 1, 1], [12, 0, 0, 40, 2])):
+        new = np.array(new)
+        total = int(new.sum())
+        kr, vr, qr = f.rows(total), f.rows(total), torch.randn(total, nh, d).to(TORCH[dtype])
+        for dst, src in ((k, kr), (v, vr), (q, qr)):
+            dst[:total] = src.cuda()
+        hd.copy_(i32(held))
+        nd.copy_(i32(new))
+        out.fill_(9.0)
+        if turn < 2:
+            step()
+        else:
+            if graph is None:
+                graph = torch.cuda.CUDAGraph()
+                torch.cuda.synchronize()
+                with torch.cuda.graph(graph):
+                    step()
+            graph.replay()
+        got, at = out.cpu().double(), 0
+        assert (got[total:] == 9).all()
+        for i in range(n):
+            m = int(new[i])
+            f.k[i].append(int(held[i]), kr[at:at + m].float().numpy())
+            f.v[i].append(int(held[i]), vr[at:at + m].float().numpy())
+            if m:
+                kw, vw = (torch.from_numpy(x.worth()).double() for x in (f.k[i], f.v[i]))
+                want, top, big = attention_f64(qr[at:at + m].double(), kw, vw, int(held[i]), d ** -0.5)
+                assert ((got[at:at + m] - want).abs() <= tolerance(want, top, big, dtype, len(kw), d)).all()
+            at += m
+        held = held + new
+    f.cache.check()
+    f.check_rows()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_gather_rows_of_a_plain_cache(cuda_device, dtype):
+    cache = llaisys.PagedKVCache(9, 2, 64, dtype=NAMES[dtype], device=llaisys.DeviceType.NVIDIA, max_seqs=2)
+    a, b = cache.add_seq(), cache.add_seq()
+    cache.assign_pages(a, [7, 2])
+    cache.assign_pages(b, [5])
+    cache.flush()
+    k, v = (torch.randn(40, 2, 64).to(TORCH[dtype]).cuda() for _ in range(2))
+    seq, pos = [a] * 30 + [b] * 10, list(range(30)) + list(range(10))
+    cache.append_dev(0, k, v, i32(seq), i32(pos), 40, stream())
+    order = torch.randperm(40)
+    out = [torch.zeros_like(k) for _ in range(2)]
+    cache.gather_dev(0, *out, i32(seq)[order.cuda()].contiguous(), i32(pos)[order.cuda()].contiguous(), 40, stream())
+    assert torch.equal(out[0], k[order.cuda()]) and torch.equal(out[1], v[order.cuda()])
+    cache.check()
+
+
+def test_gather_rows_of_a_cpu_cache():
+    cache = llaisys.PagedKVCache(9, 2, 8, dtype=llaisys.DataType.F32, max_seqs=2)
+    a = cache.add_seq()
+    cache.assign_pages(a, [7, 2])
+    k, v = torch.randn(20, 2, 8), torch.randn(20, 2, 8)
+    cache.append(0, k, v, [a] * 20, range(20))
+    out = [torch.full((3, 2, 8), 7.0) for _ in range(2)]
+    seq, pos = np.array([a, 5, a], np.int32), np.array([17, 0, 3], np.int32)
+    cache.gather_dev(0, *out, torch.from_numpy(seq), torch.from_numpy(pos), 3, None)
+    assert torch.equal(out[0][0], k[17]) and torch.equal(out[1][2], v[3]) and (out[0][1] == 7).all()
+    with pytest.raises(llaisys.LlaisysError):
+        cache.check()
+
+
+# ---- refusals --------------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("changes,status", [(dict(store=llaisys.DataType.BF16), Status.INVALID), (dict(store=llaisys.DataType.U8), Status.INVALID),
+                                            (dict(dtype=llaisys.DataType.I8), Status.INVALID), (dict(page_size=8), Status.INVALID),
+                                            (dict(page_size=24), Status.INVALID), (dict(head_dim=80), Status.INVALID),
+                                            (dict(head_dim=288), Status.INVALID), (dict(head_dim=0), Status.INVALID), (dict(nkvh=0), Status.INVALID),
+                                            (dict(num_pages=0), Status.INVALID), (dict(device=llaisys.DeviceType.CPU), Status.UNSUPPORTED),
+                                            (dict(device_id=99), Status.DEVICE)])
+def test_refusals_of_the_cache(changes, status):
+    with pytest.raises(llaisys.LlaisysError) as e:
+        llaisys.PagedKVCache.quantized(**(dict(num_pages=4, nkvh=2, head_dim=64) | changes))
+    assert e.value.status == status
+
+
+@pytest.mark.parametrize("changes,status", [(dict(held_dev=0), Status.INVALID), (dict(new_dev=0), Status.INVALID), (dict(page_size=0), Status.INVALID),
+                                            (dict(n_seqs=1 << 31), Status.INVALID), (dict(n_rows=1 << 31), Status.INVALID),
+                                            (dict(n_free=1 << 40), Status.INVALID), (dict(row_slots_dev=64), Status.INVALID),
+                                            (dict(free_pages_dev=64), Status.INVALID), (dict(table_stride=1 << 33), Status.INVALID)])
+def test_refusals_of_the_plan(changes, status):
+    args = LlaisysPagedPlan(**(dict(held_dev=64, new_dev=64, n_seqs=1, page_size=16, n_rows=1) | changes))
+    assert LIB_LLAISYS.llaisysPagedPlanDev(int(llaisys.DeviceType.NVIDIA), 0, ctypes.byref(args), None) == status
+    assert LIB_LLAISYS.llaisysPagedPlanDev(int(llaisys.DeviceType.NVIDIA), 0, None, None) == Status.INVALID
+    args = LlaisysPagedPlan(held_dev=64, new_dev=64, n_seqs=1, page_size=16, n_rows=1)
+    assert LIB_LLAISYS.llaisysPagedPlanDev(int(llaisys.DeviceType.CPU), 0, ctypes.byref(args), None) == Status.UNSUPPORTED
+
+
+@pytest.mark.gpu
+def test_refusals_of_calls_that_need_wide_pages(cuda_device):
+    f = Filled([5], 2, 128, "bf16", "i8")
+    x = torch.zeros(64, 8, 128, dtype=torch.bfloat16, device="cuda")
+    one, zero = i32([1]), i32([0])
+    calls = [lambda c: c.rope_append_dev(0, x, x, None, zero, zero, 1, 4, 1e4, stream()),
+             lambda c: c.norm_append_dev(0, stream(), proj=x, row_stride=1024, q_at=0, k_at=512, v_at=768, gate_at=-1, q_out=x, seq_ids_dev=zero,
+                                         positions_dev=zero, n_rows=1, nh=4),
+             lambda c: c.decode_step_dev(0, x, x, x, x, zero, one, 1, 1, 4, 1.0, stream()),
+             lambda c: c.decode_step_host(0, x.cpu(), x.cpu(), x.cpu(), x.cpu(), [0], [1], 4, 1.0),
+             lambda c: c.fade_dev(0, x, x, zero, None, one, n_seqs=1, total_q=1, max_q_len=1, max_kv_len=1, nh=4, scale=1.0, stream=stream(), fade_a=x,
+                                  fade_b=x),
+             lambda c: c.gates_dev(0, x, x, zero, None, one, n_seqs=1, total_q=1, max_q_len=1, max_kv_len=1, nh=4, scale=1.0, stream=stream())]
+    for call in calls:
+        with pytest.raises(llaisys.LlaisysError) as e:
+            call(f.cache)
+        assert e.value.status == Status.UNSUPPORTED
+    for call in (lambda c: c.append_dev(0, None, x, zero, zero, 1, stream()), lambda c: c.gather_dev(0, x, None, zero, zero, 1, stream()),
+                 lambda c: c.gather_dev(1, x, x, zero, zero, 1, stream()), lambda c: c.decode_dev(0, x, x, zero, one, 1, 1, 5, 1.0, stream()),
+                 lambda c: c.decode_dev(0, x, x, zero, one, 1, 1 << 20, 4, 1.0, stream())):
+        with pytest.raises(llaisys.LlaisysError) as e:
+            call(f.cache)
+        assert e.value.status == Status.INVALID
+    f.check_rows()
