@@ -165,6 +165,9 @@ PagedKV::PagedKV(const PagedKVConfig &cfg) : _cfg(cfg) {
                 _counters_len = std::max(_counters_len, counters);
             }
         }
+        if (quantized()) {
+            kernels::attention_quant_scratch(int32_t(cfg.head_dim), &_partials_floats, &_counters_len);
+        }
         if (_partials_floats != 0) {
             _partials = rt.allocateDeviceStorage(_partials_floats * sizeof(float));
             _counters = rt.allocateDeviceStorage(_counters_len * sizeof(int32_t));
