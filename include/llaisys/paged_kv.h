@@ -88,8 +88,8 @@ LLAISYS_API int llaisysPagedKVDestroy(llaisysPagedKV_t kv);
  *     s' = max(s, max|x| / M, 2^-100)   over the rows' numbers x; s only where the first of them does not go to the block's slot 0
  *     c  = round(x * (1 / s'))          to nearest, ties to even;   tokens in front of the rows, where s' > s:  c = round(c * (s * (1 / s')))
  * so that a block filled token by token is rounded again only when its scale grows. A block that a NaN or an infinity is appended to
- * gets the scale NaN, and attention of every query that reads the block is NaN, until its slot 0 is written again. Slots never written
- * read as zero.
+ * gets the scale NaN, and attention of every query that reads the block is NaN, until its slot 0 is written again. Tokens that
+ * were never written have no value.
  * The block manager, llaisysPagedKVAppend(Dev), Gather(Dev), llaisysPagedAttentionDecode(Dev), ...Prefill(Dev), ...DecodePartial(Dev) and
  * llaisysPagedAttentionOptDev (mixers.h) take such a cache with rows, queries and outputs of `dtype`; every other call returns
  * LLAISYS_E_UNSUPPORTED. The rows that one append call brings to a block must be neighbours in the call, in the order of their

@@ -30,23 +30,28 @@ namespace llaisys::kernels {
 
 namespace {
 
-constexpr int kWarps = 8, kThreads = kWarps * 32, kRows = 16;
-constexpr int kRingBytes = 132 * 1024, kMaxSlotsPerWarp = 8;
-constexpr int kMinPiece = 8; // units of the shortest piece: a block for every warp
+constexpr int kRows = 16;
+constexpr int kMinPiece = 8; // units of the shortest piece
 constexpr uint32_t kWaitLimit = 1u << 20;
 constexpr int kErrTimeout = 8;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kShift = 14.f; // weights are 2^14 times what they stand for
+constexpr size_t kPlaceBytes = 512;
 
+// Heads of up to 128: two CTAs of four warps on an SM, each warp with two blocks at a time and 255 registers. Longer ones: one CTA of eight warps.
 template <int D>
 struct Shape {
+    static constexpr int kCtas = D <= 128 ? 2 : 1, kWarps = D <= 128 ? 4 : 8, kThreads = kWarps * 32, kPair = D <= 128 ? 2 : 1;
     static constexpr int kTile = 2 * kQuantTokens * D + 16;
-    static constexpr int kSlots = kRingBytes / kWarps / kTile < kMaxSlotsPerWarp ? kRingBytes / kWarps / kTile : kMaxSlotsPerWarp; // of a warp
-    static constexpr int kMergeDims = D < 128 ? D : 128; // dims merged at a time
-    static constexpr int kMergeStride = kMergeDims + 8;  // floats between rows in the merge buffer: lanes 4 g + t store at banks 8 g + 2 t
+    static constexpr int kSlots = D <= 64 ? 8 : D <= 128 ? 4 : 2;             // of a warp
+    static constexpr int kMergeDims = D < 128 ? D : 128;                      // merged at a time
+    static constexpr int kMergeStride = kMergeDims + 8;                       // floats between rows in the merge buffer: lanes 4 g + t store at banks 8 g + 2 t
+    static constexpr int kRowThreads = kThreads / kRows, kStep = 4 * kRowThreads; // threads that load and store a row, four dims each; dims between theirs
     static constexpr size_t kMerge = size_t(kWarps) * kSlots * kTile, kStats = kMerge + size_t(kWarps) * kRows * kMergeStride * 4;
-    static constexpr size_t kBars = kStats + 3 * kWarps * kRows * 4, kWords = kBars + kWarps * kSlots * 8, kQuery = kWords + 32;
-    static constexpr size_t kBytes = kQuery + (D > 128 ? 2 * (D / 16) * 512 : 0); // (16 query rows of 256 dims stay in shared memory: 8 or 16 KiB)
+    static constexpr size_t kBars = kStats + 3 * kWarps * kRows * 4, kWords = kBars + kWarps * kSlots * 8, kPlaces = kWords + 32 + 3 * kRows * 4;
+    static constexpr size_t kQuery = kMerge; // 16 query rows as fragments, 32 bytes a dim, twice; the merge comes after their last use
+    static constexpr size_t kBytes = kPlaces + kWarps * kPlaceBytes;
+    static_assert(2 * 32 * D <= kWarps * kRows * kMergeStride * 4 && kBytes <= (kCtas == 2 ? 113 : 227) * 1024, "shared memory");
 };
 
 struct QuantParams {
@@ -61,6 +66,7 @@ struct QuantParams {
     const float *row_scale;
     int64_t out_stride;
     int32_t bf16; // of 16-bit activations: bfloat16
+    int32_t out_wide; // four outputs of a row can be stored at once
     float *partials;
     int32_t *counters;
     int32_t *error_flag;
@@ -116,79 +122,80 @@ __device__ __forceinline__ int64_t units_before(const QuantParams &p, const SeqG
     return tile + floor_sum_from(tile, g.c_hi, p.group) - (g.gaps ? floor_sum_from(tile, g.c_gap, p.group) : 0);
 }
 
-struct Fragment {
-    int a, tile, kvh;
-    int b0, b1;           // blocks of the row tile, counted without its gap; b0 = b1: none
-    int gap, kept;        // blocks left out behind the first `kept`
-    int rows;             // live rows
-    bool begins, ends;    // whether the row tile's first and last units are in it
-    int64_t first, last;  // the row tile on the line: its first unit, and the one behind its last
-    SeqGeom g;
-};
+__device__ __forceinline__ int tile_blocks(const QuantParams &p, const SeqGeom &g, int tile, int &gap) {
+    gap = g.gaps && tile + g.c_gap > 0 ? (tile + g.c_gap) / p.group : 0;
+    return (tile + g.c_hi > 0 ? (tile + g.c_hi) / p.group : 0) - gap;
+}
 
-// Place on the line; every warp walks the same fragments.
+struct Fragment {
+    int a, q_start, off, tokens; // of the sequence
+    int row0, rows, kvh;         // first packed row of the tile, live rows
+    int b0, b1;                  // blocks of the row tile, counted without its gap; b0 = b1: none
+    int kept, gap;               // gap blocks are left out behind the first `kept`
+    bool begins, ends;           // whether the row tile's first and last units are in it
+    int span;                    // units of the row tile
+    int64_t first;               // the tile's first unit on the line
+};
+// Place on the line: a row tile and kv head, and how far the piece goes.
 struct Walker {
-    int a;
-    int64_t seq_begin, pos, end;
+    int a, tile, kvh, span, gap;
+    int64_t first, pos, end;
     SeqGeom g;
-    int64_t seq_units;
 };
 __device__ __forceinline__ bool next_fragment(const QuantParams &p, Walker &w, Fragment &f) {
     if (w.pos >= w.end) {
         return false;
     }
-    while (w.pos >= w.seq_begin + w.seq_units) {
-        w.seq_begin += w.seq_units;
-        if (++w.a >= p.n_seqs) {
-            return false;
-        }
-        w.g = seq_geom(p, w.a);
-        w.seq_units = units_before(p, w.g, w.g.tiles) * p.kv.nkvh;
-    }
-    const int64_t x = w.pos - w.seq_begin;
-    int lo = 0, hi = w.g.tiles - 1; // last row tile whose first unit is not behind x
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (units_before(p, w.g, mid) * p.kv.nkvh <= x) {
-            lo = mid;
-        } else {
-            hi = mid - 1;
+    while (w.pos >= w.first + w.span) {
+        w.first += w.span;
+        if (++w.kvh == p.kv.nkvh) {
+            w.kvh = 0;
+            ++w.tile;
+            while (w.tile >= w.g.tiles) {
+                if (++w.a >= p.n_seqs) {
+                    return false;
+                }
+                w.tile = 0;
+                w.g = seq_geom(p, w.a);
+            }
+            w.span = tile_blocks(p, w.g, w.tile, w.gap) + 1;
         }
     }
-    const int64_t before = units_before(p, w.g, lo) * p.kv.nkvh;
-    const int span = int(units_before(p, w.g, int64_t(lo) + 1) - units_before(p, w.g, lo)), blocks = span - 1;
+    const int at = int(w.pos - w.first), to = int(min(int64_t(w.span), w.end - w.first));
     f.a = w.a;
-    f.tile = lo;
-    f.kvh = int((x - before) / span);
-    const int at = int(x - before - int64_t(f.kvh) * span);
-    f.first = w.seq_begin + before + int64_t(f.kvh) * span;
-    f.last = f.first + span;
-    const int to = int(min(f.last, w.end) - f.first);
+    f.q_start = w.g.q_start;
+    f.off = w.g.off;
+    f.tokens = w.g.tokens;
+    f.row0 = w.tile * kRows;
+    f.rows = min(kRows, w.g.q_len * p.group - f.row0);
+    f.kvh = w.kvh;
+    f.b0 = min(at, w.span - 1);
+    f.b1 = min(to, w.span - 1);
+    f.gap = w.gap;
+    f.kept = w.gap > 0 ? (p.keep_first + kQuantTokens - 1) / kQuantTokens : 0;
     f.begins = at == 0;
-    f.ends = to == span;
-    f.b0 = min(at, blocks);
-    f.b1 = min(to, blocks);
-    const int64_t gap = w.g.gaps && lo + w.g.c_gap > 0 ? (lo + w.g.c_gap) / p.group : 0;
-    f.gap = int(gap);
-    f.kept = gap > 0 ? (p.keep_first + kQuantTokens - 1) / kQuantTokens : 0;
-    f.rows = int(min(int64_t(kRows), int64_t(w.g.q_len) * p.group - int64_t(lo) * kRows));
-    f.g = w.g;
-    w.pos = f.first + to;
+    f.ends = to == w.span;
+    f.span = w.span;
+    f.first = w.first;
+    w.pos = w.first + to;
     return true;
 }
 
-// Four codes (a word) as two pairs of f16.
-template <bool kF8>
+// Four codes (a word) as two pairs of f16. Integers lie in the pool as u = c + 128. 0x6400 | u is 1024 + u, so 1152 less is c; the bits of u
+// alone are u 2^-24, exactly, which saves the subtraction where the caller makes good for it (kBiased).
+template <bool kF8, bool kBiased>
 __device__ __forceinline__ void widen(uint32_t w, uint32_t &lo, uint32_t &hi) {
     if constexpr (kF8) {
         const __half2_raw a = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w & 0xffffu), __NV_E4M3);
         const __half2_raw b = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w >> 16), __NV_E4M3);
         lo = uint32_t(a.x) | (uint32_t(a.y) << 16);
         hi = uint32_t(b.x) | (uint32_t(b.y) << 16);
-    } else { // 0x6400 | u is 1024 + u: with u = c + 128, 1152 less is c
-        const uint32_t u = w ^ 0x80808080u;
+    } else if constexpr (kBiased) {
+        lo = __byte_perm(w, 0, 0x4140);
+        hi = __byte_perm(w, 0, 0x4342);
+    } else {
         const __half2 off = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
-        const uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
+        const uint32_t a = __byte_perm(w, 0x64646464u, 0x4140), b = __byte_perm(w, 0x64646464u, 0x4342);
         const __half2 x = __hsub2(*reinterpret_cast<const __half2 *>(&a), off), y = __hsub2(*reinterpret_cast<const __half2 *>(&b), off);
         lo = *reinterpret_cast<const uint32_t *>(&x);
         hi = *reinterpret_cast<const uint32_t *>(&y);
@@ -208,20 +215,29 @@ __device__ __forceinline__ uint4 lds128(uint32_t addr) {
     asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
     return v;
 }
-// The blocks of a fragment that are a warp's: k-th one is block first + 8 k of the fragment. Lanes hold the tiles' places, 32 blocks at a time and
-// the next 32 ahead.
+// The blocks of a fragment that are a warp's: the warps take kPair neighbours each, in turn. Lanes hold the tiles' places, 32 blocks at a time
+// and the next 32 ahead.
 struct Feed {
     const int32_t *table; // null: no such sequence
     int count, first, kept, gap, kvh;
     int now, next;
 };
+// What a warp keeps in shared memory, off the registers of its loop over blocks.
+struct Place {
+    Walker walker;
+    Fragment ahead;
+    Feed feed; // of the fragment ahead; now and next of the lanes beside it
+    int now[32], next[32];
+};
+static_assert(sizeof(Place) <= kPlaceBytes && alignof(Place) == 8, "a warp's words");
+template <typename S>
 __device__ __forceinline__ int tile_place(const QuantParams &p, const Feed &f, int k) { // -1: no page
     if (k >= f.count) {
         return -1;
     }
-    int block = f.first + kWarps * k;
+    int block = f.first + S::kWarps * (k - k % S::kPair) + k % S::kPair;
     block = block < f.kept ? block : block + f.gap;
-    const int entry = block / p.kv.blocks_per_page;
+    const int entry = p.kv.blocks_per_page == 1 ? block : block / p.kv.blocks_per_page;
     if (f.table == nullptr || entry >= p.kv.table_stride) {
         atomicOr(p.error_flag, f.table == nullptr ? kErrBadSeq : kErrBadPosition);
         return -1;
@@ -233,17 +249,19 @@ __device__ __forceinline__ int tile_place(const QuantParams &p, const Feed &f, i
     }
     return (page * p.kv.blocks_per_page + block - entry * p.kv.blocks_per_page) * p.kv.nkvh + f.kvh;
 }
+// first: the first of the fragment's blocks that is the warp's
+template <typename S>
 __device__ __forceinline__ Feed open_feed(const QuantParams &p, const Fragment &f, int first, int lane) {
     Feed feed;
-    const int seq = p.seq_ids[f.a];
+    const int seq = p.seq_ids[f.a], blocks = f.b1 - f.b0 - first, sweep = S::kPair * S::kWarps;
     feed.table = seq >= 0 && seq < p.kv.table_rows ? p.kv.block_table + int64_t(seq) * p.kv.table_stride : nullptr;
     feed.first = f.b0 + first;
-    feed.count = max(0, (f.b1 - feed.first + kWarps - 1) / kWarps);
+    feed.count = blocks <= 0 ? 0 : blocks / sweep * S::kPair + min(blocks % sweep, S::kPair);
     feed.kept = f.kept;
     feed.gap = f.gap;
     feed.kvh = f.kvh;
-    feed.now = tile_place(p, feed, lane);
-    feed.next = tile_place(p, feed, 32 + lane);
+    feed.now = tile_place<S>(p, feed, lane);
+    feed.next = tile_place<S>(p, feed, 32 + lane);
     return feed;
 }
 
@@ -267,17 +285,51 @@ __device__ __forceinline__ float4 load4(const void *q, int64_t at, bool bf16) {
     }
 }
 
+// Four outputs of a row.
+template <bool kWide>
+__device__ __forceinline__ void store4(const QuantParams &p, int64_t at, float4 v) {
+    if constexpr (kWide) {
+        float *to = static_cast<float *>(p.out) + at;
+        if (p.out_wide) {
+            *reinterpret_cast<float4 *>(to) = v;
+        } else {
+            to[0] = v.x, to[1] = v.y, to[2] = v.z, to[3] = v.w;
+        }
+    } else {
+        uint2 w;
+        if (p.bf16) {
+            const __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
+            w = make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
+        } else {
+            w = make_uint2(pack_half2(v.x, v.y), pack_half2(v.z, v.w));
+        }
+        unsigned short *to = static_cast<unsigned short *>(p.out) + at;
+        if (p.out_wide) {
+            *reinterpret_cast<uint2 *>(to) = w;
+        } else {
+            to[0] = static_cast<unsigned short>(w.x), to[1] = static_cast<unsigned short>(w.x >> 16);
+            to[2] = static_cast<unsigned short>(w.y), to[3] = static_cast<unsigned short>(w.y >> 16);
+        }
+    }
+}
+
 // D: head dims, or the next of 64, 128 and 256 above them; kWide: 32-bit activations.
 template <int D, bool kF8, bool kWide>
-__global__ void __launch_bounds__(kThreads, 1) attention_quant_kernel(QuantParams p) {
+__global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) attention_quant_kernel(QuantParams p) {
     using S = Shape<D>;
+    constexpr int kWarps = S::kWarps, kThreads = S::kThreads, kPair = S::kPair;
     constexpr int kVecs = D / 32, kSteps = D / 16, kParts = kWide ? 2 : 1;
-    constexpr bool kQueryShared = D > 128;
+    constexpr bool kQueryRegs = !kWide && D <= 128;
+    // Integers of 16-bit activations are multiplied as u 2^-24: scores lack 128 sum q, outputs 128 sum w, both of the rounded numbers, and
+    // that is taken off in f32: 2^-23 of the largest score or value in error, which 32-bit activations do not accept.
+    constexpr bool kBiased = !kF8 && !kWide;
     extern __shared__ __align__(128) unsigned char smem[];
     float *s_merge = reinterpret_cast<float *>(smem + S::kMerge), *s_m = reinterpret_cast<float *>(smem + S::kStats);
     float *s_l = s_m + kWarps * kRows, *s_top = s_l + kWarps * kRows;
     int64_t *s_start = reinterpret_cast<int64_t *>(smem + S::kWords); // sequence of the piece's first unit, that sequence's first unit
     int *s_last = reinterpret_cast<int *>(s_start + 2);
+    float *s_factor = reinterpret_cast<float *>(s_start + 4), *s_lack = s_factor + kRows; // of the tile's rows
+    int *s_pos = reinterpret_cast<int *>(s_lack + kRows);
     uint32_t *s_query = reinterpret_cast<uint32_t *>(smem + S::kQuery); // [part][step][lane][4]
     const uint32_t query_u32 = smem_u32(s_query);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -314,7 +366,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_quant_kernel(QuantParam
         __syncthreads();
         int64_t line = 0, before = 0;
 #pragma unroll
-        for (int i = 0; i < kThreads / 32; ++i) {
+        for (int i = 0; i < kWarps; ++i) {
             before += i < warp ? sums[i] : 0;
             line += sums[i];
         }
@@ -340,226 +392,344 @@ __global__ void __launch_bounds__(kThreads, 1) attention_quant_kernel(QuantParam
         }
         __syncthreads();
         w.a = int(s_start[0]);
-        w.seq_begin = s_start[1];
         w.g = seq_geom(p, w.a);
-        w.seq_units = units_before(p, w.g, w.g.tiles) * p.kv.nkvh;
-        __syncthreads(); // the sums' place is the merge buffer's
+        const int64_t x = w.pos - s_start[1];
+        int lo = 0, hi = w.g.tiles - 1; // last row tile whose first unit is not behind x
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (units_before(p, w.g, mid) * p.kv.nkvh <= x) {
+                lo = mid;
+            } else {
+                hi = mid - 1;
+            }
+        }
+        w.tile = lo;
+        w.span = tile_blocks(p, w.g, lo, w.gap) + 1;
+        const int64_t in_front = units_before(p, w.g, lo) * p.kv.nkvh;
+        w.kvh = int(x - in_front) / w.span;
+        w.first = s_start[1] + in_front + int64_t(w.kvh) * w.span;
     }
-    Fragment f, ahead;
-    uint32_t n = 0;                  // blocks of this CTA's fragments so far: the warps take them in turn
-    uint32_t asked = 0, taken = 0;   // blocks of this warp: block c lies in slot c % kSlots
-    uint32_t found = 0;              // bit s: the page of the block in slot s exists
-    bool dead = false;               // a wait ran out
+    Place &place = *reinterpret_cast<Place *>(smem + S::kPlaces + warp * kPlaceBytes);
+    Feed feed;
+    uint32_t n = 0;                // pairs of this CTA's fragments so far: the warps take them in turn
+    uint32_t asked = 0, taken = 0; // blocks of this warp: block c lies in slot c % kSlots
+    uint32_t found = 0;            // bit s: the page of the block in slot s exists
+    bool dead = false;             // a wait ran out
+    bool more, fed_ahead = false;  // whether there is a fragment ahead, and whether the feed is its
+    int k_feed = 0;                // blocks of the feed that were asked for
     const int g = lane >> 2, t = lane & 3;
-    // asks for blocks of a feed from the k-th on, as far as there are slots
-    auto ask = [&](Feed &feed, int &k) {
-        while (k < feed.count && asked - taken < uint32_t(S::kSlots) && !dead) {
-            const int place = __shfl_sync(0xffffffffu, feed.now, k & 31);
-            const uint32_t slot = asked % S::kSlots;
-            found = place >= 0 ? found | (1u << slot) : found & ~(1u << slot);
+    // steps to the next fragment and leaves it, with its feed, in the warp's place
+    auto step = [&]() {
+        Fragment ahead;
+        const bool is = next_fragment(p, w, ahead);
+        if (is) {
+            const Feed next = open_feed<S>(p, ahead, kPair * int((uint32_t(warp) - n) & (kWarps - 1u)), lane);
+            place.now[lane] = next.now;
+            place.next[lane] = next.next;
             if (lane == 0) {
-                if (place >= 0) {
+                place.walker = w;
+                place.ahead = ahead;
+                place.feed = next;
+            }
+        }
+        __syncwarp();
+        return is;
+    };
+    // asks for blocks as far as there are slots
+    auto ask = [&]() {
+        while (asked - taken < uint32_t(S::kSlots) && !dead) {
+            if (k_feed >= feed.count) {
+                if (fed_ahead || !more) {
+                    break;
+                }
+                feed = place.feed;
+                feed.now = place.now[lane];
+                feed.next = place.next[lane];
+                fed_ahead = true;
+                k_feed = 0;
+                continue;
+            }
+            const int where = __shfl_sync(0xffffffffu, feed.now, k_feed & 31);
+            const uint32_t slot = asked % S::kSlots;
+            found = where >= 0 ? found | (1u << slot) : found & ~(1u << slot);
+            if (lane == 0) {
+                if (where >= 0) {
                     mbar_arrive_expect_tx(bars + 8 * slot, uint32_t(tile_bytes));
-                    bulk_load(ring + slot * S::kTile, p.kv.base + int64_t(place) * tile_bytes, uint32_t(tile_bytes), bars + 8 * slot);
+                    bulk_load(ring + slot * S::kTile, p.kv.base + int64_t(where) * tile_bytes, uint32_t(tile_bytes), bars + 8 * slot);
                 } else {
                     mbar_arrive(bars + 8 * slot);
                 }
             }
             ++asked;
-            if ((++k & 31) == 0) {
+            if ((++k_feed & 31) == 0) {
                 feed.now = feed.next;
-                feed.next = tile_place(p, feed, k + 32 + lane);
+                feed.next = tile_place<S>(p, feed, k_feed + 32 + lane);
             }
         }
     };
-    bool more = next_fragment(p, w, ahead);
-    Feed feed, feed_ahead = open_feed(p, ahead, warp, lane);
-    int k_feed, k_ahead = 0;
-    ask(feed_ahead, k_ahead);
-    {
-        while (more) {
-            f = ahead;
-            feed = feed_ahead;
-            k_feed = k_ahead;
-            const int first = int((uint32_t(warp) - n) & 7u);
-            n += uint32_t(f.b1 - f.b0);
-            k_ahead = 0;
-            more = next_fragment(p, w, ahead);
-            if (more) {
-                feed_ahead = open_feed(p, ahead, int((uint32_t(warp) - n) & 7u), lane);
-            } else {
-                feed_ahead.count = 0;
-            }
-            ask(feed, k_feed);
-            if (k_feed == feed.count) {
-                ask(feed_ahead, k_ahead);
-            }
-            const int kvh = f.kvh, row0 = f.tile * kRows;
-            // rows g and g + 8 of the tile: position of the query, and its fragments
-            int pos[2];
-            int64_t o_row[2]; // (query, head) as a row of out
-            float factor[2];
-            uint32_t qf[kParts][kQueryShared ? 1 : kSteps][4];
-            auto query = [&](int part, int step) -> const uint32_t(&)[4] { return qf[part][kQueryShared ? 0 : step]; };
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int r = min(g + 8 * h, f.rows - 1), packed = row0 + r, query = packed / p.group, head = packed - query * p.group;
-                pos[h] = query + f.g.off;
-                o_row[h] = int64_t(f.g.q_start + query) * p.nh + kvh * p.group + head;
-                float most = 0.f;
-#pragma unroll
-                for (int s = 0; s < kSteps; ++s) {
-                    if (s < 2 * vecs) {
-                        const float4 x = load4<kWide>(p.q, o_row[h] * d + 16 * s + 4 * t, p.bf16);
-                        most = fmaxf(most, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
-                    }
-                }
-                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-                const int e = max(-100, min(126, (__float_as_int(most) >> 23) - 127));
-                const float up = power_of_two(14 - e);
-                factor[h] = power_of_two(max(e - 14, -126)) * p.scale_log2;
-#pragma unroll
-                for (int s = 0; s < kSteps; ++s) {
-                    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (s < 2 * vecs) {
-                        x = load4<kWide>(p.q, o_row[h] * d + 16 * s + 4 * t, p.bf16);
-                    }
-                    x.x *= up, x.y *= up, x.z *= up, x.w *= up;
-                    const uint32_t lo = pack_half2(x.x, x.y), hi = pack_half2(x.z, x.w);
-                    const float2 a = rest_of(lo, x.x, x.y), b = rest_of(hi, x.z, x.w);
-                    const uint32_t parts[2][2] = {{lo, hi}, {pack_half2(a.x, a.y), pack_half2(b.x, b.y)}};
-#pragma unroll
-                    for (int part = 0; part < kParts; ++part) {
-                        if constexpr (!kQueryShared) {
-                            qf[part][s][h] = parts[part][0];
-                            qf[part][s][2 + h] = parts[part][1];
-                        } else if (s % kWarps == warp) { // every warp has read the same rows: each leaves a share of the steps
-                            uint32_t *to = s_query + ((part * kSteps + s) * 32 + lane) * 4;
-                            to[h] = parts[part][0];
-                            to[2 + h] = parts[part][1];
-                        }
-                    }
-                }
-            }
-            if constexpr (kQueryShared) {
-                __syncthreads();
-            }
-            const int first_pos = row0 / p.group + f.g.off, last_pos = (row0 + f.rows - 1) / p.group + f.g.off; // of the tile's rows
+    feed.count = 0;
+    more = step();
+    __syncthreads(); // the sums' place is the queries'
+    while (more) {
+        const Fragment f = place.ahead;
+        if (!fed_ahead) {
+            feed = place.feed;
+            feed.now = place.now[lane];
+            feed.next = place.next[lane];
+            k_feed = 0;
+        }
+        const int blocks = place.feed.count, block0 = place.feed.first; // of this warp
+        fed_ahead = false;
+        more = false;
+        ask(); // (none of the fragment behind this one)
+        n += uint32_t(f.b1 - f.b0 + kPair - 1) / kPair;
 
-            float acc[4 * kVecs][4]; // [dims 8 i ..][row g: two dims, row g + 8: two dims]
+        // ---- the tile's queries, by all threads
+        const int my_row = tid / S::kRowThreads, my_part = tid % S::kRowThreads;
+        const int my_packed = f.row0 + my_row, my_query = my_packed / p.group, my_head = f.kvh * p.group + my_packed - my_query * p.group;
+        const int64_t my_o = int64_t(f.q_start + my_query) * p.nh + my_head; // (query, head) as a row of out
+        {
+            constexpr int kPieces = D / S::kStep;
+            float4 x[kPieces];
+            float most = 0.f;
 #pragma unroll
-            for (int i = 0; i < 4 * kVecs; ++i) {
-                acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+            for (int i = 0; i < kPieces; ++i) {
+                const int dim = 4 * my_part + S::kStep * i;
+                x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (my_row < f.rows && dim < d) {
+                    x[i] = load4<kWide>(p.q, my_o * d + dim, p.bf16);
+                }
+                most = fmaxf(most, fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w))));
             }
-            float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, top[2] = {-INFINITY, -INFINITY};
-            for (int i = first; i < f.b1 - f.b0 && !dead; i += kWarps) {
-                const uint32_t slot = taken % S::kSlots;
-                if (!mbar_wait_bounded(bars + 8 * slot, (taken / S::kSlots) & 1, kWaitLimit)) {
+#pragma unroll
+            for (int o = S::kRowThreads / 2; o > 0; o >>= 1) {
+                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+            }
+            const int e = max(-100, min(126, (__float_as_int(most) >> 23) - 127));
+            const float up = power_of_two(14 - e);
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) {
+                const int dim = 4 * my_part + S::kStep * i;
+                const float4 y = make_float4(x[i].x * up, x[i].y * up, x[i].z * up, x[i].w * up);
+                const uint32_t lo = pack_half2(y.x, y.y), hi = pack_half2(y.z, y.w);
+                const float2 a = rest_of(lo, y.x, y.y), b = rest_of(hi, y.z, y.w);
+                uint32_t *to = s_query + ((dim >> 4) * 32 + 4 * (my_row & 7) + ((dim >> 2) & 3)) * 4 + (my_row >> 3);
+                to[0] = lo;
+                to[2] = hi;
+                if constexpr (kWide) {
+                    to[kSteps * 128] = pack_half2(a.x, a.y);
+                    to[kSteps * 128 + 2] = pack_half2(b.x, b.y);
+                }
+                if constexpr (kBiased) {
+                    sum += (y.x - a.x) + (y.y - a.y) + (y.z - b.x) + (y.w - b.y);
+                }
+            }
+            const float factor = power_of_two(max(e - 14, -126)) * p.scale_log2;
+            if constexpr (kBiased) {
+#pragma unroll
+                for (int o = S::kRowThreads / 2; o > 0; o >>= 1) {
+                    sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                }
+            }
+            if (my_part == 0) {
+                s_factor[my_row] = factor;
+                s_lack[my_row] = 128.f * sum * factor;
+                s_pos[my_row] = min(my_packed, f.row0 + f.rows - 1) / p.group + f.off;
+            }
+        }
+        __syncthreads();
+        float factor[2], lack[2];
+        int pos[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            factor[h] = s_factor[g + 8 * h];
+            lack[h] = s_lack[g + 8 * h];
+            pos[h] = s_pos[g + 8 * h];
+        }
+        // blocks that all of the tile's rows see all of
+        const int whole_to = min(s_pos[0], f.tokens - 1) - (kQuantTokens - 1);
+        const int whole_from = p.window > 0 ? s_pos[kRows - 1] - p.window + 1 : 0;
+        uint32_t qf[kQueryRegs ? kSteps : 1][4];
+        if constexpr (kQueryRegs) {
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+                const uint4 x = lds128(query_u32 + 16 * (i * 32 + lane));
+                qf[i][0] = x.x, qf[i][1] = x.y, qf[i][2] = x.z, qf[i][3] = x.w;
+            }
+        }
+        w = place.walker;
+        __syncwarp();
+        more = step();
+
+        // ---- its blocks
+        float acc[4 * kVecs][4]; // [dims 8 i ..][row g: two dims, row g + 8: two dims]
+#pragma unroll
+        for (int i = 0; i < 4 * kVecs; ++i) {
+            acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+        }
+        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, top[2] = {-INFINITY, -INFINITY}, weights[4] = {};
+        for (int i = 0; i < blocks && !dead; i += kPair) {
+            float s[kPair][2][4], mantissa[kPair], down[kPair], fe[kPair];
+            bool live[kPair], whole[kPair];
+#pragma unroll
+            for (int b = 0; b < kPair; ++b) {
+                live[b] = i + b < blocks && !dead;
+                if (live[b] && !mbar_wait_bounded(bars + 8 * ((taken + b) % S::kSlots), ((taken + b) / S::kSlots) & 1, kWaitLimit)) {
+                    live[b] = false;
                     dead = true;
                 }
-                dead = __any_sync(0xffffffffu, dead);
-                if (dead) {
-                    // what else is on its way lands before the CTA ends
-                    for (uint32_t c = taken; c != asked; ++c) {
-                        mbar_wait_bounded(bars + 8 * (c % S::kSlots), (c / S::kSlots) & 1, 1u << 12);
-                    }
-                    if (lane == 0) {
-                        atomicOr(p.error_flag, kErrTimeout);
-                    }
-                    break;
+            }
+            if (__any_sync(0xffffffffu, dead)) {
+                dead = true;
+                // what else is on its way lands before the CTA ends
+                for (uint32_t c = taken; c != asked; ++c) {
+                    mbar_wait_bounded(bars + 8 * (c % S::kSlots), (c / S::kSlots) & 1, 1u << 12);
                 }
-                if (found >> slot & 1) {
-                    const int k = f.b0 + i, token0 = (k < f.kept ? k : k + f.gap) * kQuantTokens;
+                if (lane == 0) {
+                    atomicOr(p.error_flag, kErrTimeout);
+                }
+                break;
+            }
+#pragma unroll
+            for (int b = 0; b < kPair; ++b) {
+                const uint32_t slot = (taken + b) % S::kSlots;
+                live[b] = live[b] && (found >> slot & 1) != 0;
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    s[b][j][0] = s[b][j][1] = s[b][j][2] = s[b][j][3] = 0.f;
+                }
+                whole[b] = false;
+                mantissa[b] = down[b] = fe[b] = 0.f;
+                if (live[b]) {
                     const uint32_t tile = ring + slot * S::kTile;
-                    const float2 scales = *reinterpret_cast<const float2 *>(my_ring + slot * S::kTile + quant_scales_at(d));
-                    float s[2][4] = {};
 #pragma unroll
                     for (int v = 0; v < kVecs; ++v) {
                         if (v < vecs) {
                             const uint4 words = lds128(tile + 16 * (32 * v + lane));
                             const uint32_t u[4] = {words.x, words.y, words.z, words.w};
 #pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                uint32_t lo, hi;
-                                widen<kF8>(u[j], lo, hi);
+                            for (int j = 0; j < 2; ++j) {
+                                uint32_t lo[2], hi[2];
+                                widen<kF8, kBiased>(u[2 * j], lo[0], hi[0]);
+                                widen<kF8, kBiased>(u[2 * j + 1], lo[1], hi[1]);
 #pragma unroll
                                 for (int part = 0; part < kParts; ++part) {
-                                    if constexpr (kQueryShared) {
-                                        if ((j & 1) == 0) {
-                                            const uint4 x = lds128(query_u32 + 16 * ((part * kSteps + 2 * v + (j >> 1)) * 32 + lane));
-                                            qf[part][0][0] = x.x, qf[part][0][1] = x.y, qf[part][0][2] = x.z, qf[part][0][3] = x.w;
-                                        }
+                                    uint32_t q[4];
+                                    if constexpr (kQueryRegs) {
+                                        q[0] = qf[2 * v + j][0], q[1] = qf[2 * v + j][1], q[2] = qf[2 * v + j][2], q[3] = qf[2 * v + j][3];
+                                    } else {
+                                        const uint4 x = lds128(query_u32 + 16 * ((part * kSteps + 2 * v + j) * 32 + lane));
+                                        q[0] = x.x, q[1] = x.y, q[2] = x.z, q[3] = x.w;
                                     }
-                                    mma_16816<false>(s[j & 1], query(part, 2 * v + (j >> 1)), lo, hi);
+                                    mma_16816<false>(s[b][0], q, lo[0], hi[0]);
+                                    mma_16816<false>(s[b][1], q, lo[1], hi[1]);
                                 }
                             }
                         }
                     }
-                    // scores in log2 units, and whether all rows see all of the block
-                    const bool whole = token0 + kQuantTokens - 1 <= first_pos && token0 + kQuantTokens <= f.g.tokens &&
-                                       (p.window == 0 || last_pos - token0 < p.window || token0 + kQuantTokens <= p.keep_first);
+                    // scores in log2 units
+                    const float2 scales = *reinterpret_cast<const float2 *>(my_ring + slot * S::kTile + quant_scales_at(d));
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const float by = factor[h] * scales.x;
+                        const float by = factor[h] * scales.x * (kBiased ? 0x1p24f : 1.f), less = kBiased ? -lack[h] * scales.x : 0.f;
 #pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-                            s[j][2 * h] *= by;
-                            s[j][2 * h + 1] *= by;
+                        for (int c = 0; c < 4; ++c) {
+                            float &x = s[b][c >> 1][2 * h + (c & 1)];
+                            x = fmaf(x, by, less);
                         }
                     }
-                    if (!whole) {
+                    int block = block0 + i * kWarps + b;
+                    block = block < f.kept ? block : block + f.gap;
+                    const int token0 = block * kQuantTokens;
+                    whole[b] = token0 <= whole_to && (token0 >= whole_from || token0 + kQuantTokens <= p.keep_first);
+                    if (!whole[b]) {
 #pragma unroll
                         for (int j = 0; j < 2; ++j) {
 #pragma unroll
                             for (int c = 0; c < 4; ++c) {
-                                const int token = token0 + 4 * t + 2 * j + (c & 1), at_pos = pos[c >> 1];
-                                const bool seen = token <= at_pos && token < f.g.tokens &&
-                                                  (p.window == 0 || at_pos - token < p.window || token < p.keep_first);
-                                s[j][c] = seen ? s[j][c] : -INFINITY;
+                                const int token = token0 + 4 * t + 2 * j + (c & 1), at = pos[c >> 1];
+                                const bool seen = token <= at && token < f.tokens && (p.window == 0 || at - token < p.window || token < p.keep_first);
+                                s[b][j][c] = seen ? s[b][j][c] : -INFINITY;
                             }
                         }
                     }
                     const int e = max(-100, min(126, ((__float_as_int(scales.y) >> 23) & 255) - 127));
-                    const float fe = float(e), mantissa = scales.y * power_of_two(-e), down = power_of_two(-e);
-                    uint32_t pf[kParts][4];
-                    float alpha[2];
+                    fe[b] = float(e);
+                    down[b] = power_of_two(-e);
+                    mantissa[b] = scales.y * down[b];
+                } else {
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        float most = fmaxf(fmaxf(s[0][2 * h], s[0][2 * h + 1]), fmaxf(s[1][2 * h], s[1][2 * h + 1]));
-                        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-                        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-                        top[h] = fmaxf(top[h], most);
-                        const float m_new = fmaxf(m[h], most + fe), base = m_new == -INFINITY ? 0.f : m_new - kShift - fe;
-                        alpha[h] = m_new == -INFINITY ? 1.f : fast_exp2(m[h] - m_new);
-                        m[h] = m_new;
-                        float x[4], sum = 0.f;
+                    for (int j = 0; j < 2; ++j) {
+                        s[b][j][0] = s[b][j][1] = s[b][j][2] = s[b][j][3] = -INFINITY;
+                    }
+                }
+            }
+            uint32_t pf[kPair][kParts][4];
+            float alpha[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float most = -INFINITY;
+#pragma unroll
+                for (int b = 0; b < kPair; ++b) {
+                    const float here = fmaxf(fmaxf(s[b][0][2 * h], s[b][0][2 * h + 1]), fmaxf(s[b][1][2 * h], s[b][1][2 * h + 1]));
+                    if (p.part != nullptr) {
+                        top[h] = fmaxf(top[h], here);
+                    }
+                    most = fmaxf(most, here + fe[b]);
+                }
+                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+                const float m_new = fmaxf(m[h], most), base = m_new == -INFINITY ? 0.f : m_new - kShift;
+                alpha[h] = m_new == -INFINITY ? 1.f : fast_exp2(m[h] - m_new);
+                m[h] = m_new;
+                l[h] *= alpha[h];
+#pragma unroll
+                for (int b = 0; b < kPair; ++b) {
+                    const float from = base - fe[b];
+                    float x[4], sum = 0.f;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        x[c] = fast_exp2(s[b][c >> 1][2 * h + (c & 1)] - from);
+                        sum += x[c];
+                    }
+                    l[h] = fmaf(sum, down[b], l[h]);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        x[c] *= mantissa[b];
+                    }
+                    if (!whole[b]) { // a lost block's NaN stays where it is seen
 #pragma unroll
                         for (int c = 0; c < 4; ++c) {
-                            x[c] = fast_exp2(s[c >> 1][2 * h + (c & 1)] - base);
-                            sum += x[c];
-                        }
-                        l[h] = l[h] * alpha[h] + sum * down;
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            x[c] = !whole && s[c >> 1][2 * h + (c & 1)] == -INFINITY ? 0.f : x[c] * mantissa; // (a lost block's NaN stays where it is seen)
-                        }
-                        pf[0][h] = pack_half2(x[0], x[1]);
-                        pf[0][2 + h] = pack_half2(x[2], x[3]);
-                        if constexpr (kWide) {
-                            const float2 a = rest_of(pf[0][h], x[0], x[1]), b = rest_of(pf[0][2 + h], x[2], x[3]);
-                            pf[1][h] = pack_half2(a.x, a.y);
-                            pf[1][2 + h] = pack_half2(b.x, b.y);
+                            x[c] = s[b][c >> 1][2 * h + (c & 1)] == -INFINITY ? 0.f : x[c];
                         }
                     }
-                    if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
+                    pf[b][0][h] = pack_half2(x[0], x[1]);
+                    pf[b][0][2 + h] = pack_half2(x[2], x[3]);
+                    if constexpr (kWide) {
+                        const float2 a = rest_of(pf[b][0][h], x[0], x[1]), r = rest_of(pf[b][0][2 + h], x[2], x[3]);
+                        pf[b][1][h] = pack_half2(a.x, a.y);
+                        pf[b][1][2 + h] = pack_half2(r.x, r.y);
+                    }
+                }
+            }
+            if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
 #pragma unroll
-                        for (int c = 0; c < 4 * kVecs; ++c) {
-                            acc[c][0] *= alpha[0];
-                            acc[c][1] *= alpha[0];
-                            acc[c][2] *= alpha[1];
-                            acc[c][3] *= alpha[1];
-                        }
+                for (int c = 0; c < 4 * kVecs; ++c) {
+                    acc[c][0] *= alpha[0];
+                    acc[c][1] *= alpha[0];
+                    acc[c][2] *= alpha[1];
+                    acc[c][3] *= alpha[1];
+                }
+                weights[0] *= alpha[0];
+                weights[2] *= alpha[1];
+            }
+#pragma unroll
+            for (int b = 0; b < kPair; ++b) {
+                if (live[b]) {
+                    const uint32_t tile = ring + ((taken + b) % S::kSlots) * S::kTile;
+                    if constexpr (kBiased) {
+                        mma_16816<false>(weights, pf[b][0], 0x3c003c00u, 0x3c003c00u); // sums of the rounded weights, against ones
                     }
 #pragma unroll
                     for (int v = 0; v < kVecs; ++v) {
@@ -569,193 +739,172 @@ __global__ void __launch_bounds__(kThreads, 1) attention_quant_kernel(QuantParam
 #pragma unroll
                             for (int j = 0; j < 4; ++j) {
                                 uint32_t lo, hi;
-                                widen<kF8>(u[j], lo, hi);
-                                mma_16816<false>(acc[4 * v + j], pf[0], lo, hi);
-                                if constexpr (kWide) {
-                                    mma_16816<false>(acc[4 * v + j], pf[1], lo, hi);
+                                widen<kF8, kBiased>(u[j], lo, hi);
+#pragma unroll
+                                for (int part = 0; part < kParts; ++part) {
+                                    mma_16816<false>(acc[4 * v + j], pf[b][part], lo, hi);
                                 }
                             }
                         }
                     }
                 }
-                __syncwarp();
-                ++taken;
-                ask(feed, k_feed);
-                if (k_feed == feed.count) {
-                    ask(feed_ahead, k_ahead);
-                }
             }
+            __syncwarp();
+            taken += uint32_t(min(kPair, blocks - i));
+            ask();
+        }
 
-            // ---- the eight warps' sums
+        // ---- the warps' sums
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-                l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-                if (t == 0) {
-                    s_m[warp * kRows + g + 8 * h] = m[h];
-                    s_l[warp * kRows + g + 8 * h] = l[h];
-                    s_top[warp * kRows + g + 8 * h] = top[h];
-                }
+        for (int h = 0; h < 2; ++h) {
+            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+            if (p.part != nullptr) {
+                top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
+                top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
             }
-            __syncthreads();
-            float share[2];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                float all = -INFINITY;
-#pragma unroll
-                for (int i = 0; i < kWarps; ++i) {
-                    all = fmaxf(all, s_m[i * kRows + g + 8 * h]);
-                }
-                share[h] = all == -INFINITY ? 1.f : fast_exp2(m[h] - all);
+            if (t == 0) {
+                s_m[warp * kRows + g + 8 * h] = m[h];
+                s_l[warp * kRows + g + 8 * h] = l[h];
+                s_top[warp * kRows + g + 8 * h] = top[h];
             }
-            const bool whole_tile = f.begins && f.ends;
-            float *slot_of_mine = p.partials + (int64_t(blockIdx.x) * 2 + (f.begins ? 1 : 0)) * partial_floats(d);
-            // statistics of the tile's rows, by every thread for the row it stores
-            const int out_row = tid >> 4, out_lane = tid & 15;
-            float m_all = -INFINITY, l_all = 0.f, top_all = -INFINITY;
+        }
+        __syncthreads();
+        float share[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float all = -INFINITY;
 #pragma unroll
             for (int i = 0; i < kWarps; ++i) {
-                m_all = fmaxf(m_all, s_m[i * kRows + out_row]);
-                top_all = fmaxf(top_all, s_top[i * kRows + out_row]);
+                all = fmaxf(all, s_m[i * kRows + g + 8 * h]);
             }
+            share[h] = all == -INFINITY ? 1.f : fast_exp2(m[h] - all);
+        }
+        float m_all = -INFINITY, l_all = 0.f, top_all = -INFINITY; // of the row that this thread stores
 #pragma unroll
-            for (int i = 0; i < kWarps; ++i) {
-                l_all += s_l[i * kRows + out_row] * (m_all == -INFINITY ? 1.f : fast_exp2(s_m[i * kRows + out_row] - m_all));
+        for (int i = 0; i < kWarps; ++i) {
+            m_all = fmaxf(m_all, s_m[i * kRows + my_row]);
+            top_all = fmaxf(top_all, s_top[i * kRows + my_row]);
+        }
+#pragma unroll
+        for (int i = 0; i < kWarps; ++i) {
+            l_all += s_l[i * kRows + my_row] * (m_all == -INFINITY ? 1.f : fast_exp2(s_m[i * kRows + my_row] - m_all));
+        }
+        const bool whole_tile = f.begins && f.ends;
+        float *slot_of_mine = p.partials + (int64_t(blockIdx.x) * 2 + (f.begins ? 1 : 0)) * partial_floats(d);
+        const float gate = p.row_scale != nullptr && my_row < f.rows && p.part == nullptr ? p.row_scale[my_o] : 1.f;
+        const int64_t my_out = int64_t(f.q_start + my_query) * p.out_stride + int64_t(my_head) * d;
+        // a finished row's numbers
+        auto finish = [&](int dim, float4 v, float by) {
+            v.x *= by, v.y *= by, v.z *= by, v.w *= by;
+            if (p.part != nullptr) {
+                float *to = p.part + my_o * (d + 2) + dim;
+                to[0] = v.x, to[1] = v.y, to[2] = v.z, to[3] = v.w;
+            } else {
+                store4<kWide>(p, my_out + dim, v);
             }
+        };
+        auto finish_stats = [&](float m_row, float l_row, float top_row) {
+            if (p.part != nullptr && my_part == 0 && my_row < f.rows) {
+                float *to = p.part + my_o * (d + 2) + d;
+                to[0] = top_row * kLn2;
+                to[1] = top_row == -INFINITY ? l_row : l_row * fast_exp2(m_row - kShift - top_row);
+            }
+        };
+        const float by = (l_all == 0.f ? 0.f : 1.f / l_all) * gate;
 #pragma unroll
-            for (int c0 = 0; c0 < D; c0 += S::kMergeDims) {
-                if (c0 < d) {
+        for (int c0 = 0; c0 < D; c0 += S::kMergeDims) {
+            if (c0 < d) {
 #pragma unroll
-                    for (int i = 0; i < S::kMergeDims / 8; ++i) {
-                        const float *x = acc[c0 / 8 + i];
-                        float *at = s_merge + (warp * kRows + g) * S::kMergeStride + 8 * i + 2 * t;
-                        *reinterpret_cast<float2 *>(at) = make_float2(x[0] * share[0], x[1] * share[0]);
-                        *reinterpret_cast<float2 *>(at + 8 * S::kMergeStride) = make_float2(x[2] * share[1], x[3] * share[1]);
+                for (int i = 0; i < S::kMergeDims / 8; ++i) {
+                    float x[4];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        x[c] = acc[c0 / 8 + i][c];
+                        if constexpr (kBiased) {
+                            x[c] = fmaf(x[c], 0x1p24f, -128.f * weights[c & 2]);
+                        }
+                        x[c] *= share[c >> 1];
                     }
-                    __syncthreads();
-                    const float inv = l_all == 0.f ? 0.f : 1.f / l_all;
-                    const int packed = row0 + out_row, query = packed / p.group, head = packed - query * p.group;
-                    const int64_t row = int64_t(f.g.q_start + query), o = row * p.nh + kvh * p.group + head;
+                    float *at = s_merge + (warp * kRows + g) * S::kMergeStride + 8 * i + 2 * t;
+                    *reinterpret_cast<float2 *>(at) = make_float2(x[0], x[1]);
+                    *reinterpret_cast<float2 *>(at + 8 * S::kMergeStride) = make_float2(x[2], x[3]);
+                }
+                __syncthreads();
 #pragma unroll
-                    for (int i = 0; i < S::kMergeDims / 64; ++i) { // four dims at a time
-                        const int dim = 64 * i + 4 * out_lane;
-                        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+                for (int i = 0; i < S::kMergeDims / S::kStep; ++i) {
+                    const int dim = S::kStep * i + 4 * my_part;
+                    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-                        for (int k = 0; k < kWarps; ++k) {
-                            const float4 x = *reinterpret_cast<const float4 *>(s_merge + (k * kRows + out_row) * S::kMergeStride + dim);
-                            sum.x += x.x, sum.y += x.y, sum.z += x.z, sum.w += x.w;
-                        }
-                        if (c0 + dim >= d) {
-                            continue;
-                        }
+                    for (int k = 0; k < kWarps; ++k) {
+                        const float4 x = *reinterpret_cast<const float4 *>(s_merge + (k * kRows + my_row) * S::kMergeStride + dim);
+                        sum.x += x.x, sum.y += x.y, sum.z += x.z, sum.w += x.w;
+                    }
+                    if (c0 + dim < d) {
                         if (!whole_tile) {
-                            __stcg(reinterpret_cast<float4 *>(slot_of_mine + out_row * d + c0 + dim), sum);
-                        } else if (out_row < f.rows) {
-                            sum.x *= inv, sum.y *= inv, sum.z *= inv, sum.w *= inv;
-                            if (p.part != nullptr) {
-                                float *to = p.part + o * (d + 2) + c0 + dim;
-                                to[0] = sum.x, to[1] = sum.y, to[2] = sum.z, to[3] = sum.w;
-                            } else {
-                                const float by = p.row_scale != nullptr ? p.row_scale[o] : 1.f;
-                                const int64_t to = row * p.out_stride + int64_t(kvh * p.group + head) * d + c0 + dim;
-                                const float v[4] = {sum.x * by, sum.y * by, sum.z * by, sum.w * by};
-#pragma unroll
-                                for (int k = 0; k < 4; ++k) {
-                                    if constexpr (kWide) {
-                                        static_cast<float *>(p.out)[to + k] = v[k];
-                                    } else if (p.bf16) {
-                                        static_cast<__nv_bfloat16 *>(p.out)[to + k] = __float2bfloat16_rn(v[k]);
-                                    } else {
-                                        static_cast<__half *>(p.out)[to + k] = __float2half_rn(v[k]);
-                                    }
-                                }
-                            }
+                            __stcg(reinterpret_cast<float4 *>(slot_of_mine + my_row * d + c0 + dim), sum);
+                        } else if (my_row < f.rows) {
+                            finish(c0 + dim, sum, by);
                         }
                     }
-                    __syncthreads(); // the buffer is free again
                 }
+                __syncthreads(); // the buffer is free again
             }
-            if (whole_tile) {
-                if (p.part != nullptr && out_lane == 0 && out_row < f.rows) {
-                    const int packed = row0 + out_row, query = packed / p.group, head = packed - query * p.group;
-                    float *to = p.part + (int64_t(f.g.q_start + query) * p.nh + kvh * p.group + head) * (d + 2) + d;
-                    to[0] = top_all * kLn2;
-                    to[1] = top_all == -INFINITY ? l_all : l_all * fast_exp2(m_all - kShift - top_all);
-                }
-                continue;
-            }
-            // ---- one of several fragments of its tile
-            if (out_lane == 0) {
-                float *stats = slot_of_mine + kRows * d;
-                __stcg(stats + out_row, m_all);
-                __stcg(stats + kRows + out_row, l_all);
-                __stcg(stats + 2 * kRows + out_row, top_all);
-            }
-            const int c_first = int(f.first / piece), c_last = int((f.last - 1) / piece);
-            __threadfence();
-            __syncthreads();
-            if (tid == 0) {
-                const int seen = atomicAdd(p.counters + c_first, 1);
-                *s_last = seen == c_last - c_first;
-                if (*s_last) {
-                    p.counters[c_first] = 0;
-                }
-            }
-            __syncthreads();
+        }
+        if (whole_tile) {
+            finish_stats(m_all, l_all, top_all);
+            continue;
+        }
+        // ---- one of several fragments of its tile
+        if (my_part == 0) {
+            float *stats = slot_of_mine + kRows * d;
+            __stcg(stats + my_row, m_all);
+            __stcg(stats + kRows + my_row, l_all);
+            __stcg(stats + 2 * kRows + my_row, top_all);
+        }
+        const int c_first = int(f.first / piece), c_last = int((f.first + f.span - 1) / piece);
+        __threadfence();
+        __syncthreads();
+        if (tid == 0) {
+            const int seen = atomicAdd(p.counters + c_first, 1);
+            *s_last = seen == c_last - c_first;
             if (*s_last) {
-                __threadfence();
-                float m_tile = -INFINITY, l_tile = 0.f, top_tile = -INFINITY;
-                for (int c = c_first; c <= c_last; ++c) {
-                    const float *stats = p.partials + (int64_t(c) * 2 + (c == c_first ? 1 : 0)) * partial_floats(d) + kRows * d;
-                    m_tile = fmaxf(m_tile, __ldcg(stats + out_row));
-                    top_tile = fmaxf(top_tile, __ldcg(stats + 2 * kRows + out_row));
-                }
-                float4 sum[D / 64] = {};
-                for (int c = c_first; c <= c_last; ++c) {
-                    const float *from = p.partials + (int64_t(c) * 2 + (c == c_first ? 1 : 0)) * partial_floats(d);
-                    const float by = m_tile == -INFINITY ? 1.f : fast_exp2(__ldcg(from + kRows * d + out_row) - m_tile);
-                    l_tile += __ldcg(from + kRows * d + kRows + out_row) * by;
+                p.counters[c_first] = 0;
+            }
+        }
+        __syncthreads();
+        if (*s_last) {
+            __threadfence();
+            float m_tile = -INFINITY, l_tile = 0.f, top_tile = -INFINITY;
+            for (int c = c_first; c <= c_last; ++c) {
+                const float *stats = p.partials + (int64_t(c) * 2 + (c == c_first ? 1 : 0)) * partial_floats(d) + kRows * d;
+                m_tile = fmaxf(m_tile, __ldcg(stats + my_row));
+                top_tile = fmaxf(top_tile, __ldcg(stats + 2 * kRows + my_row));
+            }
+            float4 sum[D / S::kStep] = {};
+            for (int c = c_first; c <= c_last; ++c) {
+                const float *from = p.partials + (int64_t(c) * 2 + (c == c_first ? 1 : 0)) * partial_floats(d);
+                const float to = m_tile == -INFINITY ? 1.f : fast_exp2(__ldcg(from + kRows * d + my_row) - m_tile);
+                l_tile += __ldcg(from + kRows * d + kRows + my_row) * to;
 #pragma unroll
-                    for (int i = 0; i < D / 64; ++i) {
-                        const int dim = 64 * i + 4 * out_lane;
-                        if (dim < d) {
-                            const float4 x = __ldcg(reinterpret_cast<const float4 *>(from + out_row * d + dim));
-                            sum[i].x += x.x * by, sum[i].y += x.y * by, sum[i].z += x.z * by, sum[i].w += x.w * by;
-                        }
-                    }
-                }
-                if (out_row < f.rows) {
-                    const float inv = l_tile == 0.f ? 0.f : 1.f / l_tile;
-                    const int packed = row0 + out_row, query = packed / p.group, head = packed - query * p.group;
-                    const int64_t row = int64_t(f.g.q_start + query), o = row * p.nh + kvh * p.group + head;
-                    const float by = inv * (p.row_scale != nullptr && p.part == nullptr ? p.row_scale[o] : 1.f);
-#pragma unroll
-                    for (int i = 0; i < D / 64; ++i) {
-                        const int dim = 64 * i + 4 * out_lane;
-                        if (dim < d) {
-                            const float v[4] = {sum[i].x * by, sum[i].y * by, sum[i].z * by, sum[i].w * by};
-                            const int64_t to = row * p.out_stride + int64_t(kvh * p.group + head) * d + dim;
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                if (p.part != nullptr) {
-                                    p.part[o * (d + 2) + dim + k] = v[k];
-                                } else if constexpr (kWide) {
-                                    static_cast<float *>(p.out)[to + k] = v[k];
-                                } else if (p.bf16) {
-                                    static_cast<__nv_bfloat16 *>(p.out)[to + k] = __float2bfloat16_rn(v[k]);
-                                } else {
-                                    static_cast<__half *>(p.out)[to + k] = __float2half_rn(v[k]);
-                                }
-                            }
-                        }
-                    }
-                    if (p.part != nullptr && out_lane == 0) {
-                        float *to = p.part + o * (d + 2) + d;
-                        to[0] = top_tile * kLn2;
-                        to[1] = top_tile == -INFINITY ? l_tile : l_tile * fast_exp2(m_tile - kShift - top_tile);
+                for (int i = 0; i < D / S::kStep; ++i) {
+                    const int dim = S::kStep * i + 4 * my_part;
+                    if (dim < d) {
+                        const float4 x = __ldcg(reinterpret_cast<const float4 *>(from + my_row * d + dim));
+                        sum[i].x += x.x * to, sum[i].y += x.y * to, sum[i].z += x.z * to, sum[i].w += x.w * to;
                     }
                 }
             }
+            if (my_row < f.rows) {
+                const float by_tile = (l_tile == 0.f ? 0.f : 1.f / l_tile) * gate;
+#pragma unroll
+                for (int i = 0; i < D / S::kStep; ++i) {
+                    if (S::kStep * i + 4 * my_part < d) {
+                        finish(S::kStep * i + 4 * my_part, sum[i], by_tile);
+                    }
+                }
+            }
+            finish_stats(m_tile, l_tile, top_tile);
         }
     }
 }
@@ -763,8 +912,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_quant_kernel(QuantParam
 } // namespace
 
 void attention_quant_scratch(int32_t d, size_t *floats, size_t *counters) {
-    *floats = size_t(device_sms()) * 2 * partial_floats(d);
-    *counters = size_t(device_sms());
+    const size_t ctas = size_t(device_sms()) * (d <= 128 ? Shape<128>::kCtas : Shape<256>::kCtas);
+    *floats = ctas * 2 * partial_floats(d);
+    *counters = ctas;
 }
 
 void attention_quant(stream_t stream, llaisysDataType_t dtype, const QuantView &kv, const AttnBatch &batch, const void *q, float scale,
@@ -787,18 +937,20 @@ void attention_quant(stream_t stream, llaisysDataType_t dtype, const QuantView &
     p.row_scale = out.row_scale;
     p.out_stride = out.row_stride ? out.row_stride : int64_t(batch.nh) * kv.d;
     p.bf16 = dtype == LLAISYS_DTYPE_BF16;
+    p.out_wide = reinterpret_cast<uintptr_t>(out.out) % (dtype == LLAISYS_DTYPE_F32 ? 16 : 8) == 0 && p.out_stride % 4 == 0;
     p.partials = scratch.partials;
     p.counters = scratch.counters;
     p.error_flag = scratch.error_flag;
-    const unsigned sms = unsigned(device_sms());
     CHECK_ARGUMENT(aligned16(q), "attention: queries must be 16-byte aligned");
     CHECK_ARGUMENT(int64_t(batch.total_q) * p.group <= 0x7fffffff - kRows, "attention: too many rows for one launch");
-    CHECK_ARGUMENT(scratch.partials_floats >= size_t(sms) * 2 * partial_floats(kv.d) && scratch.counters_len >= sms, "attention: workspace too small");
+    size_t floats, counters;
+    attention_quant_scratch(kv.d, &floats, &counters);
+    CHECK_ARGUMENT(scratch.partials_floats >= floats && scratch.counters_len >= counters, "attention: workspace too small");
     auto launch = [&](auto d) {
         constexpr int D = decltype(d)::value;
         auto start = [&](auto kernel) {
             LLAISYS_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(Shape<D>::kBytes)));
-            kernel<<<sms, kThreads, Shape<D>::kBytes, static_cast<cudaStream_t>(stream)>>>(p);
+            kernel<<<unsigned(counters), Shape<D>::kThreads, Shape<D>::kBytes, static_cast<cudaStream_t>(stream)>>>(p);
         };
         if (dtype == LLAISYS_DTYPE_F32) {
             start(kv.f8 ? attention_quant_kernel<D, true, true> : attention_quant_kernel<D, false, true>);

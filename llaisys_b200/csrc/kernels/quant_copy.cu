@@ -74,7 +74,7 @@ __global__ void __launch_bounds__(128) quant_append_kernel(QuantView kv, const T
         for (int r = 0; r < run; ++r) {
             for (int x = lane; x < d; x += 32) {
                 codes[is_v ? quant_v_at(slot + r, x) : quant_k_at(slot + r, x)] =
-                    finite ? quant_code<kF8>(to_f32(rows[r * row_step + x]) * inverse) : static_cast<unsigned char>(0);
+                    quant_code<kF8>(finite ? to_f32(rows[r * row_step + x]) * inverse : 0.f);
             }
         }
         __syncwarp();

@@ -29,13 +29,13 @@ __host__ __device__ __forceinline__ int quant_v_at(int token, int dim) { // from
 }
 __host__ __device__ __forceinline__ int quant_scales_at(int d) { return 2 * kQuantTokens * d; }
 
-// Codes of a store: kF8 = e4m3, else integers.
+// Codes of a store: kF8 = e4m3, else integers c, kept as c + 128.
 template <bool kF8>
 __device__ __forceinline__ unsigned char quant_code(float x) {
     if constexpr (kF8) {
         return __nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3);
     } else {
-        return static_cast<unsigned char>(static_cast<signed char>(max(-127, min(127, __float2int_rn(x)))));
+        return static_cast<unsigned char>(128 + max(-127, min(127, __float2int_rn(x))));
     }
 }
 template <bool kF8>
@@ -43,7 +43,7 @@ __device__ __forceinline__ float quant_worth(unsigned char c) {
     if constexpr (kF8) {
         return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3)));
     } else {
-        return float(static_cast<signed char>(c));
+        return float(int(c) - 128);
     }
 }
 
