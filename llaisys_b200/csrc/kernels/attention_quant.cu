@@ -31,7 +31,9 @@ namespace llaisys::kernels {
 namespace {
 
 constexpr int kRows = 16;
-constexpr int kMinPiece = 8; // units of the shortest piece
+constexpr int kMinPiece = 16; // units of the shortest piece
+constexpr int kTileUnits = 12; // what a row tile costs besides its blocks, in units of a block's time
+constexpr int kSnap = 8;       // a piece's border that comes this near a row tile's first or last block moves there: no fragments of a few blocks
 constexpr uint32_t kWaitLimit = 1u << 20;
 constexpr int kErrTimeout = 8;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
@@ -49,9 +51,11 @@ struct Shape {
     static constexpr int kRowThreads = kThreads / kRows, kStep = 4 * kRowThreads; // threads that load and store a row, four dims each; dims between theirs
     static constexpr size_t kMerge = size_t(kWarps) * kSlots * kTile, kStats = kMerge + size_t(kWarps) * kRows * kMergeStride * 4;
     static constexpr size_t kBars = kStats + 3 * kWarps * kRows * 4, kWords = kBars + kWarps * kSlots * 8, kPlaces = kWords + 32 + 3 * kRows * 4;
+    static constexpr size_t kPending = kPlaces + kWarps * kPlaceBytes; // fragments of tiles that other CTAs have parts of: at most two
+    static constexpr size_t kRaw = kPending + 256;                     // the next tile's query rows as they are
     static constexpr size_t kQuery = kMerge; // 16 query rows as fragments, 32 bytes a dim, twice; the merge comes after their last use
-    static constexpr size_t kBytes = kPlaces + kWarps * kPlaceBytes;
-    static_assert(2 * 32 * D <= kWarps * kRows * kMergeStride * 4 && kBytes <= (kCtas == 2 ? 113 : 227) * 1024, "shared memory");
+    static constexpr size_t bytes(bool wide) { return kRaw + kRows * D * (wide ? 4 : 2); }
+    static_assert(2 * 32 * D <= kWarps * kRows * kMergeStride * 4 && bytes(true) <= (kCtas == 2 ? 113 : 227) * 1024 && kRaw % 16 == 0, "");
 };
 
 struct QuantParams {
@@ -119,7 +123,7 @@ __device__ __forceinline__ int64_t units_before(const QuantParams &p, const SeqG
     if (tile == 0) {
         return 0;
     }
-    return tile + floor_sum_from(tile, g.c_hi, p.group) - (g.gaps ? floor_sum_from(tile, g.c_gap, p.group) : 0);
+    return kTileUnits * tile + floor_sum_from(tile, g.c_hi, p.group) - (g.gaps ? floor_sum_from(tile, g.c_gap, p.group) : 0);
 }
 
 __device__ __forceinline__ int tile_blocks(const QuantParams &p, const SeqGeom &g, int tile, int &gap) {
@@ -132,53 +136,62 @@ struct Fragment {
     int row0, rows, kvh;         // first packed row of the tile, live rows
     int b0, b1;                  // blocks of the row tile, counted without its gap; b0 = b1: none
     int kept, gap;               // gap blocks are left out behind the first `kept`
-    bool begins, ends;           // whether the row tile's first and last units are in it
-    int span;                    // units of the row tile
+    bool begins, ends;           // whether the row tile's first and last blocks are in it
+    int blocks;                  // of the row tile
     int64_t first;               // the tile's first unit on the line
 };
 // Place on the line: a row tile and kv head, and how far the piece goes.
 struct Walker {
-    int a, tile, kvh, span, gap;
+    int a, tile, kvh, blocks, gap;
     int64_t first, pos, end;
     SeqGeom g;
 };
+__device__ __forceinline__ int snap_of(int blocks) { return min(kSnap, blocks / 2); }
+// where in a row tile a border lies that is x units behind its first
+__device__ __forceinline__ int snapped(int64_t x, int blocks) {
+    const int near = snap_of(blocks);
+    return x <= near ? 0 : x >= blocks - near ? blocks + kTileUnits : int(x);
+}
 __device__ __forceinline__ bool next_fragment(const QuantParams &p, Walker &w, Fragment &f) {
-    if (w.pos >= w.end) {
-        return false;
-    }
-    while (w.pos >= w.first + w.span) {
-        w.first += w.span;
-        if (++w.kvh == p.kv.nkvh) {
-            w.kvh = 0;
-            ++w.tile;
-            while (w.tile >= w.g.tiles) {
-                if (++w.a >= p.n_seqs) {
-                    return false;
+    while (w.pos < w.end) {
+        while (w.pos >= w.first + w.blocks + kTileUnits) {
+            w.first += w.blocks + kTileUnits;
+            if (++w.kvh == p.kv.nkvh) {
+                w.kvh = 0;
+                ++w.tile;
+                while (w.tile >= w.g.tiles) {
+                    if (++w.a >= p.n_seqs) {
+                        return false;
+                    }
+                    w.tile = 0;
+                    w.g = seq_geom(p, w.a);
                 }
-                w.tile = 0;
-                w.g = seq_geom(p, w.a);
+                w.blocks = tile_blocks(p, w.g, w.tile, w.gap);
             }
-            w.span = tile_blocks(p, w.g, w.tile, w.gap) + 1;
         }
+        const int span = w.blocks + kTileUnits, at = snapped(w.pos - w.first, w.blocks), to = snapped(w.end - w.first, w.blocks);
+        w.pos = w.first + span;
+        if (at >= to) {
+            continue; // the neighbours' pieces take it
+        }
+        f.a = w.a;
+        f.q_start = w.g.q_start;
+        f.off = w.g.off;
+        f.tokens = w.g.tokens;
+        f.row0 = w.tile * kRows;
+        f.rows = min(kRows, w.g.q_len * p.group - f.row0);
+        f.kvh = w.kvh;
+        f.b0 = at;
+        f.b1 = min(to, w.blocks);
+        f.gap = w.gap;
+        f.kept = w.gap > 0 ? (p.keep_first + kQuantTokens - 1) / kQuantTokens : 0;
+        f.begins = at == 0;
+        f.ends = to == span;
+        f.blocks = w.blocks;
+        f.first = w.first;
+        return true;
     }
-    const int at = int(w.pos - w.first), to = int(min(int64_t(w.span), w.end - w.first));
-    f.a = w.a;
-    f.q_start = w.g.q_start;
-    f.off = w.g.off;
-    f.tokens = w.g.tokens;
-    f.row0 = w.tile * kRows;
-    f.rows = min(kRows, w.g.q_len * p.group - f.row0);
-    f.kvh = w.kvh;
-    f.b0 = min(at, w.span - 1);
-    f.b1 = min(to, w.span - 1);
-    f.gap = w.gap;
-    f.kept = w.gap > 0 ? (p.keep_first + kQuantTokens - 1) / kQuantTokens : 0;
-    f.begins = at == 0;
-    f.ends = to == w.span;
-    f.span = w.span;
-    f.first = w.first;
-    w.pos = w.first + to;
-    return true;
+    return false;
 }
 
 // Four codes (a word) as two pairs of f16. Integers lie in the pool as u = c + 128. 0x6400 | u is 1024 + u, so 1152 less is c; the bits of u
@@ -229,7 +242,7 @@ struct Place {
     Feed feed; // of the fragment ahead; now and next of the lanes beside it
     int now[32], next[32];
 };
-static_assert(sizeof(Place) <= kPlaceBytes && alignof(Place) == 8, "a warp's words");
+static_assert(sizeof(Place) <= kPlaceBytes && alignof(Place) == 8 && 2 * sizeof(Fragment) <= 256, "shared memory");
 template <typename S>
 __device__ __forceinline__ int tile_place(const QuantParams &p, const Feed &f, int k) { // -1: no page
     if (k >= f.count) {
@@ -269,13 +282,13 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
                  : "memory");
 }
-// Four neighbouring elements of a query row.
+// Four neighbouring elements of a query row in shared memory.
 template <bool kWide>
-__device__ __forceinline__ float4 load4(const void *q, int64_t at, bool bf16) {
+__device__ __forceinline__ float4 load4(const unsigned char *q, int at, bool bf16) {
     if constexpr (kWide) {
-        return *reinterpret_cast<const float4 *>(static_cast<const float *>(q) + at);
+        return *reinterpret_cast<const float4 *>(q + 4 * at);
     } else {
-        const uint2 w = *reinterpret_cast<const uint2 *>(static_cast<const unsigned short *>(q) + at);
+        const uint2 w = *reinterpret_cast<const uint2 *>(q + 2 * at);
         if (bf16) {
             return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16),
                                __uint_as_float(w.y & 0xffff0000u));
@@ -313,8 +326,27 @@ __device__ __forceinline__ void store4(const QuantParams &p, int64_t at, float4 
     }
 }
 
-// D: head dims, or the next of 64, 128 and 256 above them; kWide: 32-bit activations.
-template <int D, bool kF8, bool kWide>
+// Four numbers of a finished row `o` ((query, head)), and a partial result's statistics.
+template <bool kWide>
+__device__ __forceinline__ void finish(const QuantParams &p, int64_t o, int64_t out_at, int dim, float4 v, float by) {
+    v.x *= by, v.y *= by, v.z *= by, v.w *= by;
+    if (p.part != nullptr) {
+        float *to = p.part + o * (p.kv.d + 2) + dim;
+        to[0] = v.x, to[1] = v.y, to[2] = v.z, to[3] = v.w;
+    } else {
+        store4<kWide>(p, out_at + dim, v);
+    }
+}
+__device__ __forceinline__ void finish_stats(const QuantParams &p, int64_t o, float m, float l, float top) {
+    if (p.part != nullptr) {
+        float *to = p.part + o * (p.kv.d + 2) + p.kv.d;
+        to[0] = top * kLn2;
+        to[1] = top == -INFINITY ? l : l * fast_exp2(m - kShift - top);
+    }
+}
+
+// D: head dims, or (kExact false) the next of 64, 128 and 256 above them; kWide: 32-bit activations.
+template <int D, bool kExact, bool kF8, bool kWide>
 __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) attention_quant_kernel(QuantParams p) {
     using S = Shape<D>;
     constexpr int kWarps = S::kWarps, kThreads = S::kThreads, kPair = S::kPair;
@@ -333,7 +365,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) attention
     uint32_t *s_query = reinterpret_cast<uint32_t *>(smem + S::kQuery); // [part][step][lane][4]
     const uint32_t query_u32 = smem_u32(s_query);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int d = p.kv.d, vecs = d >> 5, tile_bytes = p.kv.tile_bytes;
+    const int d = kExact ? D : p.kv.d, vecs = d >> 5, tile_bytes = 2 * kQuantTokens * d + 16;
     unsigned char *my_ring = smem + size_t(warp) * S::kSlots * S::kTile;
     const uint32_t ring = smem_u32(my_ring), bars = smem_u32(smem + S::kBars) + uint32_t(warp) * S::kSlots * 8;
 
@@ -404,25 +436,38 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) attention
             }
         }
         w.tile = lo;
-        w.span = tile_blocks(p, w.g, lo, w.gap) + 1;
+        w.blocks = tile_blocks(p, w.g, lo, w.gap);
         const int64_t in_front = units_before(p, w.g, lo) * p.kv.nkvh;
-        w.kvh = int(x - in_front) / w.span;
-        w.first = s_start[1] + in_front + int64_t(w.kvh) * w.span;
+        w.kvh = int(x - in_front) / (w.blocks + kTileUnits);
+        w.first = s_start[1] + in_front + int64_t(w.kvh) * (w.blocks + kTileUnits);
     }
     Place &place = *reinterpret_cast<Place *>(smem + S::kPlaces + warp * kPlaceBytes);
     Feed feed;
     uint32_t n = 0;                // pairs of this CTA's fragments so far: the warps take them in turn
     uint32_t asked = 0, taken = 0; // blocks of this warp: block c lies in slot c % kSlots
+    Fragment *s_pending = reinterpret_cast<Fragment *>(smem + S::kPending);
+    int pending = 0;
     uint32_t found = 0;            // bit s: the page of the block in slot s exists
     bool dead = false;             // a wait ran out
     bool more, fed_ahead = false;  // whether there is a fragment ahead, and whether the feed is its
     int k_feed = 0;                // blocks of the feed that were asked for
     const int g = lane >> 2, t = lane & 3;
-    // steps to the next fragment and leaves it, with its feed, in the warp's place
+    const int my_row = tid / S::kRowThreads, my_part = tid % S::kRowThreads; // the row of a tile that this thread loads and stores a share of
+    unsigned char *s_raw = smem + S::kRaw;
+    // steps to the next fragment and leaves it, with its feed, in the warp's place; its queries are on their way
     auto step = [&]() {
         Fragment ahead;
         const bool is = next_fragment(p, w, ahead);
         if (is) {
+            constexpr int kElem = kWide ? 4 : 2;
+            if (my_row < ahead.rows) {
+                const int packed = ahead.row0 + my_row, query = packed / p.group, head = ahead.kvh * p.group + packed - query * p.group;
+                const unsigned char *from = static_cast<const unsigned char *>(p.q) + (int64_t(ahead.q_start + query) * p.nh + head) * d * kElem;
+                for (int at = 16 * my_part; at < d * kElem; at += 16 * S::kRowThreads) {
+                    cp_async_16(smem_u32(s_raw) + my_row * D * kElem + at, from + at, 16);
+                }
+            }
+            cp_async_commit();
             const Feed next = open_feed<S>(p, ahead, kPair * int((uint32_t(warp) - n) & (kWarps - 1u)), lane);
             place.now[lane] = next.now;
             place.next[lane] = next.next;
@@ -480,15 +525,16 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) attention
         }
         const int blocks = place.feed.count, block0 = place.feed.first; // of this warp
         fed_ahead = false;
-        more = false;
-        ask(); // (none of the fragment behind this one)
         n += uint32_t(f.b1 - f.b0 + kPair - 1) / kPair;
 
         // ---- the tile's queries, by all threads
-        const int my_row = tid / S::kRowThreads, my_part = tid % S::kRowThreads;
         const int my_packed = f.row0 + my_row, my_query = my_packed / p.group, my_head = f.kvh * p.group + my_packed - my_query * p.group;
         const int64_t my_o = int64_t(f.q_start + my_query) * p.nh + my_head; // (query, head) as a row of out
         {
+            more = false;
+            ask(); // (none of the fragment behind this one)
+            cp_async_wait<0>();
+            __syncthreads();
             constexpr int kPieces = D / S::kStep;
             float4 x[kPieces];
             float most = 0.f;
@@ -497,7 +543,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) attention
                 const int dim = 4 * my_part + S::kStep * i;
                 x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
                 if (my_row < f.rows && dim < d) {
-                    x[i] = load4<kWide>(p.q, my_o * d + dim, p.bf16);
+                    x[i] = load4<kWide>(s_raw, my_row * D + dim, p.bf16);
                 }
                 most = fmaxf(most, fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w))));
             }
@@ -571,14 +617,13 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) attention
         float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, top[2] = {-INFINITY, -INFINITY}, weights[4] = {};
         for (int i = 0; i < blocks && !dead; i += kPair) {
             float s[kPair][2][4], mantissa[kPair], down[kPair], fe[kPair];
-            bool live[kPair], whole[kPair];
+            uint32_t slot[kPair]; // (the block behind the last one is the last one again, with nothing seen of it: no branch between the two)
+            bool live[kPair];
 #pragma unroll
             for (int b = 0; b < kPair; ++b) {
-                live[b] = i + b < blocks && !dead;
-                if (live[b] && !mbar_wait_bounded(bars + 8 * ((taken + b) % S::kSlots), ((taken + b) / S::kSlots) & 1, kWaitLimit)) {
-                    live[b] = false;
-                    dead = true;
-                }
+                live[b] = i + b < blocks;
+                slot[b] = (taken + (live[b] ? b : 0)) % S::kSlots;
+                dead = dead || !mbar_wait_bounded(bars + 8 * slot[b], ((taken + (live[b] ? b : 0)) / S::kSlots) & 1, kWaitLimit);
             }
             if (__any_sync(0xffffffffu, dead)) {
                 dead = true;
@@ -591,77 +636,92 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) attention
                 }
                 break;
             }
+            bool whole = true;
+            int token0[kPair];
 #pragma unroll
             for (int b = 0; b < kPair; ++b) {
-                const uint32_t slot = (taken + b) % S::kSlots;
-                live[b] = live[b] && (found >> slot & 1) != 0;
+                int block = block0 + i * kWarps + b;
+                block = block < f.kept ? block : block + f.gap;
+                token0[b] = block * kQuantTokens;
+                if ((found >> slot[b] & 1) == 0) { // no page: nothing seen of it, and nothing odd in its place
+                    live[b] = false;
+                    for (int at = 16 * lane; at < tile_bytes; at += 512) {
+                        *reinterpret_cast<uint4 *>(my_ring + slot[b] * S::kTile + at) = make_uint4(0, 0, 0, 0);
+                    }
+                    __syncwarp();
+                }
+                whole = whole && live[b] && token0[b] <= whole_to && (token0[b] >= whole_from || token0[b] + kQuantTokens <= p.keep_first);
+            }
+#pragma unroll
+            for (int b = 0; b < kPair; ++b) {
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     s[b][j][0] = s[b][j][1] = s[b][j][2] = s[b][j][3] = 0.f;
                 }
-                whole[b] = false;
-                mantissa[b] = down[b] = fe[b] = 0.f;
-                if (live[b]) {
-                    const uint32_t tile = ring + slot * S::kTile;
+            }
 #pragma unroll
-                    for (int v = 0; v < kVecs; ++v) {
-                        if (v < vecs) {
-                            const uint4 words = lds128(tile + 16 * (32 * v + lane));
-                            const uint32_t u[4] = {words.x, words.y, words.z, words.w};
+            for (int v = 0; v < kVecs; ++v) {
+                if (v < vecs) {
+                    uint32_t u[kPair][4];
 #pragma unroll
-                            for (int j = 0; j < 2; ++j) {
-                                uint32_t lo[2], hi[2];
-                                widen<kF8, kBiased>(u[2 * j], lo[0], hi[0]);
-                                widen<kF8, kBiased>(u[2 * j + 1], lo[1], hi[1]);
-#pragma unroll
-                                for (int part = 0; part < kParts; ++part) {
-                                    uint32_t q[4];
-                                    if constexpr (kQueryRegs) {
-                                        q[0] = qf[2 * v + j][0], q[1] = qf[2 * v + j][1], q[2] = qf[2 * v + j][2], q[3] = qf[2 * v + j][3];
-                                    } else {
-                                        const uint4 x = lds128(query_u32 + 16 * ((part * kSteps + 2 * v + j) * 32 + lane));
-                                        q[0] = x.x, q[1] = x.y, q[2] = x.z, q[3] = x.w;
-                                    }
-                                    mma_16816<false>(s[b][0], q, lo[0], hi[0]);
-                                    mma_16816<false>(s[b][1], q, lo[1], hi[1]);
-                                }
-                            }
-                        }
+                    for (int b = 0; b < kPair; ++b) {
+                        const uint4 words = lds128(ring + slot[b] * S::kTile + 16 * (32 * v + lane));
+                        u[b][0] = words.x, u[b][1] = words.y, u[b][2] = words.z, u[b][3] = words.w;
                     }
-                    // scores in log2 units
-                    const float2 scales = *reinterpret_cast<const float2 *>(my_ring + slot * S::kTile + quant_scales_at(d));
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const float by = factor[h] * scales.x * (kBiased ? 0x1p24f : 1.f), less = kBiased ? -lack[h] * scales.x : 0.f;
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            float &x = s[b][c >> 1][2 * h + (c & 1)];
-                            x = fmaf(x, by, less);
-                        }
-                    }
-                    int block = block0 + i * kWarps + b;
-                    block = block < f.kept ? block : block + f.gap;
-                    const int token0 = block * kQuantTokens;
-                    whole[b] = token0 <= whole_to && (token0 >= whole_from || token0 + kQuantTokens <= p.keep_first);
-                    if (!whole[b]) {
-#pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-#pragma unroll
-                            for (int c = 0; c < 4; ++c) {
-                                const int token = token0 + 4 * t + 2 * j + (c & 1), at = pos[c >> 1];
-                                const bool seen = token <= at && token < f.tokens && (p.window == 0 || at - token < p.window || token < p.keep_first);
-                                s[b][j][c] = seen ? s[b][j][c] : -INFINITY;
-                            }
-                        }
-                    }
-                    const int e = max(-100, min(126, ((__float_as_int(scales.y) >> 23) & 255) - 127));
-                    fe[b] = float(e);
-                    down[b] = power_of_two(-e);
-                    mantissa[b] = scales.y * down[b];
-                } else {
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        s[b][j][0] = s[b][j][1] = s[b][j][2] = s[b][j][3] = -INFINITY;
+                        uint32_t q[kParts][4];
+#pragma unroll
+                        for (int part = 0; part < kParts; ++part) {
+                            if constexpr (kQueryRegs) {
+                                q[part][0] = qf[2 * v + j][0], q[part][1] = qf[2 * v + j][1], q[part][2] = qf[2 * v + j][2], q[part][3] = qf[2 * v + j][3];
+                            } else {
+                                const uint4 x = lds128(query_u32 + 16 * ((part * kSteps + 2 * v + j) * 32 + lane));
+                                q[part][0] = x.x, q[part][1] = x.y, q[part][2] = x.z, q[part][3] = x.w;
+                            }
+                        }
+#pragma unroll
+                        for (int b = 0; b < kPair; ++b) {
+                            uint32_t lo[2], hi[2];
+                            widen<kF8, kBiased>(u[b][2 * j], lo[0], hi[0]);
+                            widen<kF8, kBiased>(u[b][2 * j + 1], lo[1], hi[1]);
+#pragma unroll
+                            for (int part = 0; part < kParts; ++part) {
+                                mma_16816<false>(s[b][0], q[part], lo[0], hi[0]);
+                                mma_16816<false>(s[b][1], q[part], lo[1], hi[1]);
+                            }
+                        }
+                    }
+                }
+            }
+#pragma unroll
+            for (int b = 0; b < kPair; ++b) { // scores in log2 units
+                const float2 scales = *reinterpret_cast<const float2 *>(my_ring + slot[b] * S::kTile + quant_scales_at(d));
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float by = factor[h] * scales.x * (kBiased ? 0x1p24f : 1.f), less = kBiased ? -lack[h] * scales.x : 0.f;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        float &x = s[b][c >> 1][2 * h + (c & 1)];
+                        x = fmaf(x, by, less);
+                    }
+                }
+                const int e = max(-100, min(126, ((__float_as_int(scales.y) >> 23) & 255) - 127));
+                fe[b] = float(e);
+                down[b] = power_of_two(-e);
+                mantissa[b] = scales.y * down[b];
+            }
+            if (!whole) {
+#pragma unroll
+                for (int b = 0; b < kPair; ++b) {
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            const int token = token0[b] + 4 * t + 2 * j + (c & 1), at = pos[c >> 1];
+                            const bool seen = live[b] && token <= at && token < f.tokens && (p.window == 0 || at - token < p.window || token < p.keep_first);
+                            s[b][j][c] = seen ? s[b][j][c] : -INFINITY;
+                        }
                     }
                 }
             }
@@ -673,9 +733,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) attention
 #pragma unroll
                 for (int b = 0; b < kPair; ++b) {
                     const float here = fmaxf(fmaxf(s[b][0][2 * h], s[b][0][2 * h + 1]), fmaxf(s[b][1][2 * h], s[b][1][2 * h + 1]));
-                    if (p.part != nullptr) {
-                        top[h] = fmaxf(top[h], here);
-                    }
+                    top[h] = fmaxf(top[h], here);
                     most = fmaxf(most, here + fe[b]);
                 }
                 most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
@@ -698,7 +756,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) attention
                     for (int c = 0; c < 4; ++c) {
                         x[c] *= mantissa[b];
                     }
-                    if (!whole[b]) { // a lost block's NaN stays where it is seen
+                    if (!whole) { // a lost block's NaN stays where it is seen
 #pragma unroll
                         for (int c = 0; c < 4; ++c) {
                             x[c] = s[b][c >> 1][2 * h + (c & 1)] == -INFINITY ? 0.f : x[c];
@@ -726,24 +784,21 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) attention
             }
 #pragma unroll
             for (int b = 0; b < kPair; ++b) {
-                if (live[b]) {
-                    const uint32_t tile = ring + ((taken + b) % S::kSlots) * S::kTile;
-                    if constexpr (kBiased) {
-                        mma_16816<false>(weights, pf[b][0], 0x3c003c00u, 0x3c003c00u); // sums of the rounded weights, against ones
-                    }
+                if constexpr (kBiased) {
+                    mma_16816<false>(weights, pf[b][0], 0x3c003c00u, 0x3c003c00u); // sums of the rounded weights, against ones
+                }
 #pragma unroll
-                    for (int v = 0; v < kVecs; ++v) {
-                        if (v < vecs) {
-                            const uint4 words = lds128(tile + kQuantTokens * d + 16 * (32 * v + lane));
-                            const uint32_t u[4] = {words.x, words.y, words.z, words.w};
+                for (int v = 0; v < kVecs; ++v) {
+                    if (v < vecs) {
+                        const uint4 words = lds128(ring + slot[b] * S::kTile + kQuantTokens * d + 16 * (32 * v + lane));
+                        const uint32_t u[4] = {words.x, words.y, words.z, words.w};
 #pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                uint32_t lo, hi;
-                                widen<kF8, kBiased>(u[j], lo, hi);
+                        for (int j = 0; j < 4; ++j) {
+                            uint32_t lo, hi;
+                            widen<kF8, kBiased>(u[j], lo, hi);
 #pragma unroll
-                                for (int part = 0; part < kParts; ++part) {
-                                    mma_16816<false>(acc[4 * v + j], pf[b][part], lo, hi);
-                                }
+                            for (int part = 0; part < kParts; ++part) {
+                                mma_16816<false>(acc[4 * v + j], pf[b][part], lo, hi);
                             }
                         }
                     }
@@ -794,23 +849,6 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) attention
         float *slot_of_mine = p.partials + (int64_t(blockIdx.x) * 2 + (f.begins ? 1 : 0)) * partial_floats(d);
         const float gate = p.row_scale != nullptr && my_row < f.rows && p.part == nullptr ? p.row_scale[my_o] : 1.f;
         const int64_t my_out = int64_t(f.q_start + my_query) * p.out_stride + int64_t(my_head) * d;
-        // a finished row's numbers
-        auto finish = [&](int dim, float4 v, float by) {
-            v.x *= by, v.y *= by, v.z *= by, v.w *= by;
-            if (p.part != nullptr) {
-                float *to = p.part + my_o * (d + 2) + dim;
-                to[0] = v.x, to[1] = v.y, to[2] = v.z, to[3] = v.w;
-            } else {
-                store4<kWide>(p, my_out + dim, v);
-            }
-        };
-        auto finish_stats = [&](float m_row, float l_row, float top_row) {
-            if (p.part != nullptr && my_part == 0 && my_row < f.rows) {
-                float *to = p.part + my_o * (d + 2) + d;
-                to[0] = top_row * kLn2;
-                to[1] = top_row == -INFINITY ? l_row : l_row * fast_exp2(m_row - kShift - top_row);
-            }
-        };
         const float by = (l_all == 0.f ? 0.f : 1.f / l_all) * gate;
 #pragma unroll
         for (int c0 = 0; c0 < D; c0 += S::kMergeDims) {
@@ -844,7 +882,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) attention
                         if (!whole_tile) {
                             __stcg(reinterpret_cast<float4 *>(slot_of_mine + my_row * d + c0 + dim), sum);
                         } else if (my_row < f.rows) {
-                            finish(c0 + dim, sum, by);
+                            finish<kWide>(p, my_o, my_out, c0 + dim, sum, by);
                         }
                     }
                 }
@@ -852,59 +890,76 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) attention
             }
         }
         if (whole_tile) {
-            finish_stats(m_all, l_all, top_all);
-            continue;
+            if (my_part == 0 && my_row < f.rows) {
+                finish_stats(p, my_o, m_all, l_all, top_all);
+            }
+        } else {
+            if (my_part == 0) {
+                float *stats = slot_of_mine + kRows * d;
+                __stcg(stats + my_row, m_all);
+                __stcg(stats + kRows + my_row, l_all);
+                __stcg(stats + 2 * kRows + my_row, top_all);
+            }
+            if (tid == 0) {
+                s_pending[pending] = f;
+            }
+            ++pending;
         }
-        // ---- one of several fragments of its tile
-        if (my_part == 0) {
-            float *stats = slot_of_mine + kRows * d;
-            __stcg(stats + my_row, m_all);
-            __stcg(stats + kRows + my_row, l_all);
-            __stcg(stats + 2 * kRows + my_row, top_all);
-        }
-        const int c_first = int(f.first / piece), c_last = int((f.first + f.span - 1) / piece);
-        __threadfence();
-        __syncthreads();
+    }
+
+    // ---- tiles that other CTAs have parts of: whoever comes last puts the parts together, in the order of the CTAs
+    __syncthreads();
+    for (int k = 0; k < pending; ++k) {
+        const Fragment f = s_pending[k];
+        const int c_first = int((f.first + snap_of(f.blocks)) / piece), c_last = int((f.first + f.blocks - snap_of(f.blocks) - 1) / piece);
         if (tid == 0) {
+            __threadfence(); // (of everybody's parts: they were written before the barrier)
             const int seen = atomicAdd(p.counters + c_first, 1);
             *s_last = seen == c_last - c_first;
             if (*s_last) {
                 p.counters[c_first] = 0;
             }
+            __threadfence();
         }
         __syncthreads();
-        if (*s_last) {
-            __threadfence();
-            float m_tile = -INFINITY, l_tile = 0.f, top_tile = -INFINITY;
-            for (int c = c_first; c <= c_last; ++c) {
-                const float *stats = p.partials + (int64_t(c) * 2 + (c == c_first ? 1 : 0)) * partial_floats(d) + kRows * d;
-                m_tile = fmaxf(m_tile, __ldcg(stats + my_row));
-                top_tile = fmaxf(top_tile, __ldcg(stats + 2 * kRows + my_row));
-            }
-            float4 sum[D / S::kStep] = {};
-            for (int c = c_first; c <= c_last; ++c) {
-                const float *from = p.partials + (int64_t(c) * 2 + (c == c_first ? 1 : 0)) * partial_floats(d);
-                const float to = m_tile == -INFINITY ? 1.f : fast_exp2(__ldcg(from + kRows * d + my_row) - m_tile);
-                l_tile += __ldcg(from + kRows * d + kRows + my_row) * to;
+        const bool last = *s_last != 0;
+        __syncthreads();
+        if (!last) {
+            continue;
+        }
+        const int my_packed = f.row0 + my_row, my_query = my_packed / p.group, my_head = f.kvh * p.group + my_packed - my_query * p.group;
+        const int64_t my_o = int64_t(f.q_start + my_query) * p.nh + my_head, my_out = int64_t(f.q_start + my_query) * p.out_stride + int64_t(my_head) * d;
+        float m_tile = -INFINITY, l_tile = 0.f, top_tile = -INFINITY;
+        for (int c = c_first; c <= c_last; ++c) {
+            const float *stats = p.partials + (int64_t(c) * 2 + (c == c_first ? 1 : 0)) * partial_floats(d) + kRows * d;
+            m_tile = fmaxf(m_tile, __ldcg(stats + my_row));
+            top_tile = fmaxf(top_tile, __ldcg(stats + 2 * kRows + my_row));
+        }
+        float4 sum[D / S::kStep] = {};
+        for (int c = c_first; c <= c_last; ++c) {
+            const float *from = p.partials + (int64_t(c) * 2 + (c == c_first ? 1 : 0)) * partial_floats(d);
+            const float to = m_tile == -INFINITY ? 1.f : fast_exp2(__ldcg(from + kRows * d + my_row) - m_tile);
+            l_tile += __ldcg(from + kRows * d + kRows + my_row) * to;
 #pragma unroll
-                for (int i = 0; i < D / S::kStep; ++i) {
-                    const int dim = S::kStep * i + 4 * my_part;
-                    if (dim < d) {
-                        const float4 x = __ldcg(reinterpret_cast<const float4 *>(from + my_row * d + dim));
-                        sum[i].x += x.x * to, sum[i].y += x.y * to, sum[i].z += x.z * to, sum[i].w += x.w * to;
-                    }
+            for (int i = 0; i < D / S::kStep; ++i) {
+                const int dim = S::kStep * i + 4 * my_part;
+                if (dim < d) {
+                    const float4 x = __ldcg(reinterpret_cast<const float4 *>(from + my_row * d + dim));
+                    sum[i].x += x.x * to, sum[i].y += x.y * to, sum[i].z += x.z * to, sum[i].w += x.w * to;
                 }
             }
-            if (my_row < f.rows) {
-                const float by_tile = (l_tile == 0.f ? 0.f : 1.f / l_tile) * gate;
+        }
+        if (my_row < f.rows) {
+            const float by = (l_tile == 0.f ? 0.f : 1.f / l_tile) * (p.row_scale != nullptr && p.part == nullptr ? p.row_scale[my_o] : 1.f);
 #pragma unroll
-                for (int i = 0; i < D / S::kStep; ++i) {
-                    if (S::kStep * i + 4 * my_part < d) {
-                        finish(S::kStep * i + 4 * my_part, sum[i], by_tile);
-                    }
+            for (int i = 0; i < D / S::kStep; ++i) {
+                if (S::kStep * i + 4 * my_part < d) {
+                    finish<kWide>(p, my_o, my_out, S::kStep * i + 4 * my_part, sum[i], by);
                 }
             }
-            finish_stats(m_tile, l_tile, top_tile);
+            if (my_part == 0) {
+                finish_stats(p, my_o, m_tile, l_tile, top_tile);
+            }
         }
     }
 }
@@ -949,13 +1004,22 @@ void attention_quant(stream_t stream, llaisysDataType_t dtype, const QuantView &
     auto launch = [&](auto d) {
         constexpr int D = decltype(d)::value;
         auto start = [&](auto kernel) {
-            LLAISYS_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(Shape<D>::kBytes)));
-            kernel<<<unsigned(counters), Shape<D>::kThreads, Shape<D>::kBytes, static_cast<cudaStream_t>(stream)>>>(p);
+            const size_t bytes = Shape<D>::bytes(dtype == LLAISYS_DTYPE_F32);
+            LLAISYS_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes)));
+            kernel<<<unsigned(counters), Shape<D>::kThreads, bytes, static_cast<cudaStream_t>(stream)>>>(p);
         };
-        if (dtype == LLAISYS_DTYPE_F32) {
-            start(kv.f8 ? attention_quant_kernel<D, true, true> : attention_quant_kernel<D, false, true>);
+        auto pick = [&](auto exact) {
+            constexpr bool kExact = decltype(exact)::value;
+            if (dtype == LLAISYS_DTYPE_F32) {
+                start(kv.f8 ? attention_quant_kernel<D, kExact, true, true> : attention_quant_kernel<D, kExact, false, true>);
+            } else {
+                start(kv.f8 ? attention_quant_kernel<D, kExact, true, false> : attention_quant_kernel<D, kExact, false, false>);
+            }
+        };
+        if (kv.d == D) {
+            pick(std::true_type{});
         } else {
-            start(kv.f8 ? attention_quant_kernel<D, true, false> : attention_quant_kernel<D, false, false>);
+            pick(std::false_type{});
         }
     };
     if (kv.d <= 64) {
