@@ -76,6 +76,9 @@ struct PlanArgs {
     int32_t *q_starts = nullptr, *kv_lens = nullptr, *page_starts = nullptr, *row_seqs = nullptr, *row_positions = nullptr;
     int64_t *row_slots = nullptr;
     int32_t *status = nullptr;
+    // set by the launcher
+    int32_t page_shift = -1; // page_size = 1 << page_shift
+    bool rows_wide = false;  // row arrays can be stored 16 bytes at a time
 };
 
 // Which queries attend to which sequences. Arrays live on the executing device; a null array selects the

@@ -1,25 +1,35 @@
 // The index arrays of a step from its requests' lengths: sums of what is in front of every request, then for every row its request, token and
 // slot, and for every new page its entry of the block table.
 //
-// One CTA goes through the requests 1024 at a time (a sum over the warp, one over the warps, a carry), then over rows and pages, which find
-// their request by bisection of the sums.
+// Bound: a launch for batches that decode, bytes (16 a row, 8 a page) for prompts. One launch, and no CTA waits for another: every CTA sums all
+// requests by itself -- a CHUNK of neighbours per thread, a sum over warps and CTA -- and then writes its share of the rows, four at a time
+// per thread, and of the requests. A row finds its chunk by bisection of the chunks' sums in shared memory and its request by walking the
+// chunk. (Handing the sums from CTA to CTA would read the lengths once instead of once per CTA; they are 8 bytes a request out of L2.)
+// 64 requests of one token: 30.8 us a call with one CTA that went through its requests one by one, of which the launch itself was a part; 4000
+// prompts of 1 to 512 tokens (a million rows): 2530 us with that kernel.
 #include "kernels.hpp"
 #include "launch_utils.cuh"
 
 #include "llaisys/paged_kv.h"
 
+#include <algorithm>
 #include <climits>
 
 namespace llaisys::kernels {
 
 namespace {
 
-constexpr int kThreads = 1024;
+constexpr int kRowsAtOnce = 4;
 
 struct Request {
     int row, held, fresh; // table row (-1: not in the table), tokens held and brought
+    int held_pages, pages, grown;
 };
 
+__device__ __forceinline__ int pages_of(int tokens, const PlanArgs &p) {
+    return p.page_shift >= 0 ? int((uint32_t(tokens) + uint32_t(p.page_size) - 1u) >> p.page_shift)
+                             : int((uint32_t(tokens) + uint32_t(p.page_size) - 1u) / uint32_t(p.page_size));
+}
 __device__ __forceinline__ Request load_request(const PlanArgs &p, int i, int &flags) {
     Request q;
     q.row = p.seq_ids ? p.seq_ids[i] : i;
@@ -34,145 +44,221 @@ __device__ __forceinline__ Request load_request(const PlanArgs &p, int i, int &f
         flags |= LLAISYS_PLAN_BAD_ROW;
         q.row = -1;
     }
+    q.held_pages = pages_of(q.held, p);
+    q.pages = pages_of(q.held + q.fresh, p);
+    q.grown = 0;
+    if (p.free_pages != nullptr && q.row >= 0 && q.fresh > 0) {
+        if (q.pages > p.table_stride) {
+            flags |= LLAISYS_PLAN_BAD_ROW;
+        } else {
+            q.grown = q.pages - q.held_pages;
+        }
+    }
     return q;
 }
-__device__ __forceinline__ int pages_of(int tokens, int page_size) { return int((int64_t(tokens) + page_size - 1) / page_size); }
-// pages a request takes off the free list
-__device__ __forceinline__ int growth(const PlanArgs &p, const Request &q, int &flags) {
-    if (p.free_pages == nullptr || q.row < 0 || q.fresh == 0) {
-        return 0;
+
+// The last chunk whose sum in front is not over x (chunks that add nothing in front of it are passed over).
+template <int kChunks, typename T>
+__device__ __forceinline__ int chunk_of(const T *sums, int64_t x) {
+    int lo = 0, hi = kChunks - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (sums[mid] <= x) {
+            lo = mid;
+        } else {
+            hi = mid - 1;
+        }
     }
-    const int after = pages_of(q.held + q.fresh, p.page_size);
-    if (after > p.table_stride) {
-        flags |= LLAISYS_PLAN_BAD_ROW;
-        return 0;
-    }
-    return after - pages_of(q.held, p.page_size);
+    return lo;
 }
 
-// Exclusive sum over the CTA of three numbers; `carry` comes in as the sum of what is in front and leaves with this lot's added.
-__device__ __forceinline__ void scan3(int64_t (&v)[3], int64_t (&carry)[3], int64_t (*sums)[3]) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int64_t own[3];
-#pragma unroll
-    for (int k = 0; k < 3; ++k) {
-        own[k] = v[k];
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int64_t up = __shfl_up_sync(0xffffffffu, v[k], o);
-            v[k] += lane >= o ? up : 0;
-        }
-        if (lane == 31) {
-            sums[warp][k] = v[k];
-        }
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < 3; ++k) {
-        int64_t before = 0, all = 0;
-        for (int w = 0; w < kThreads / 32; ++w) {
-            before += w < warp ? sums[w][k] : 0;
-            all += sums[w][k];
-        }
-        v[k] = carry[k] + before + v[k] - own[k];
-        carry[k] += all;
-    }
-    __syncthreads();
-}
-
+template <int kThreads>
 __global__ void __launch_bounds__(kThreads) paged_plan_kernel(PlanArgs p) {
-    __shared__ int64_t s_sums[kThreads / 32][3];
+    constexpr int kWarps = kThreads / 32;
+    __shared__ int64_t s_warp[kWarps][3];
+    __shared__ int64_t s_rows[kThreads]; // rows in front of a chunk
+    __shared__ int s_grown[kThreads];    // pages taken in front of it
     __shared__ int s_flags;
-    if (threadIdx.x == 0) {
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid == 0) {
         s_flags = 0;
     }
-    __syncthreads();
+    const int per = (p.n_seqs + kThreads - 1) / kThreads, i0 = min(tid * per, p.n_seqs), i1 = min(i0 + per, p.n_seqs);
     int flags = 0;
-    // totals first: pages are taken all or not at all
-    int64_t total[3] = {0, 0, 0};
-    for (int base = 0; base < p.n_seqs; base += kThreads) {
-        const int i = base + int(threadIdx.x);
-        int64_t v[3] = {0, 0, 0};
-        if (i < p.n_seqs) {
-            const Request q = load_request(p, i, flags);
-            v[2] = growth(p, q, flags);
+    int64_t mine[3] = {0, 0, 0}; // rows, pages, pages taken
+    for (int i = i0; i < i1; ++i) {
+        const Request q = load_request(p, i, flags);
+        mine[0] += q.fresh;
+        mine[1] += q.pages;
+        mine[2] += q.grown;
+    }
+    int64_t before[3] = {mine[0], mine[1], mine[2]};
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+            const int64_t up = __shfl_up_sync(0xffffffffu, before[k], o);
+            before[k] += lane >= o ? up : 0;
         }
-        scan3(v, total, s_sums);
+    }
+    if (lane == 31) {
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+            s_warp[warp][k] = before[k];
+        }
+    }
+    __syncthreads();
+    if (flags != 0) {
+        atomicOr(&s_flags, flags);
+    }
+    if (warp == 0) {
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+            int64_t v = lane < kWarps ? s_warp[lane][k] : 0;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int64_t up = __shfl_up_sync(0xffffffffu, v, o);
+                v += lane >= o ? up : 0;
+            }
+            if (lane < kWarps) {
+                s_warp[lane][k] = v;
+            }
+        }
+    }
+    __syncthreads();
+    int64_t total[3];
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+        before[k] += (warp > 0 ? s_warp[warp - 1][k] : 0) - mine[k];
+        total[k] = s_warp[kWarps - 1][k];
     }
     const bool enough = total[2] <= p.n_free;
-    int64_t carry[3] = {0, 0, 0};
-    for (int base = 0; base < p.n_seqs; base += kThreads) {
-        const int i = base + int(threadIdx.x);
-        int64_t v[3] = {0, 0, 0};
-        Request q{-1, 0, 0};
-        int grown = 0;
-        if (i < p.n_seqs) {
-            q = load_request(p, i, flags);
-            grown = growth(p, q, flags);
-            v[0] = q.fresh;
-            v[1] = pages_of(q.held + q.fresh, p.page_size);
-            v[2] = grown;
-        }
-        scan3(v, carry, s_sums);
-        if (i < p.n_seqs) {
-            const int first = int(min(v[0], int64_t(p.n_rows)));
+    s_rows[tid] = before[0];
+    s_grown[tid] = int(min(before[2], int64_t(INT_MAX)));
+    __syncthreads();
+
+    // ---- this CTA's share of the requests, by warps: what is said about each
+    if (warp * int(gridDim.x) / kWarps == int(blockIdx.x)) {
+        int64_t rows = before[0], pages = before[1];
+        for (int i = i0; i < i1; ++i) {
+            const Request q = load_request(p, i, flags);
             if (p.q_starts) {
-                p.q_starts[i] = first;
+                p.q_starts[i] = int(min(rows, int64_t(p.n_rows)));
             }
             if (p.kv_lens) {
                 p.kv_lens[i] = q.held + q.fresh;
             }
             if (p.page_starts) {
-                p.page_starts[i] = int(min(v[1], int64_t(INT_MAX)));
+                p.page_starts[i] = int(min(pages, int64_t(INT_MAX)));
             }
-            const int held_pages = pages_of(q.held, p.page_size);
-            if (enough) {
-                for (int k = 0; k < grown; ++k) {
-                    p.table[int64_t(q.row) * p.table_stride + held_pages + k] = p.free_pages[v[2] + k];
-                }
-            }
-            const int rows = int(min(v[0] + q.fresh, int64_t(p.n_rows))) - first;
-            for (int r = 0; r < rows; ++r) {
-                const int pos = q.held + r, entry = pos / p.page_size;
-                if (p.row_seqs) {
-                    p.row_seqs[first + r] = p.seq_ids ? p.seq_ids[i] : i;
-                }
-                if (p.row_positions) {
-                    p.row_positions[first + r] = pos;
-                }
-                if (p.row_slots) {
-                    int page = -1;
-                    if (q.row >= 0 && entry < p.table_stride && (entry < held_pages || p.free_pages == nullptr || (enough && grown > 0))) {
-                        page = p.table[int64_t(q.row) * p.table_stride + entry];
-                    }
-                    p.row_slots[first + r] = page < 0 ? -1 : int64_t(page) * p.page_size + (pos - entry * p.page_size);
-                }
-            }
+            rows += q.fresh;
+            pages += q.pages;
         }
     }
-    for (int r = int(min(carry[0], int64_t(p.n_rows))) + int(threadIdx.x); r < p.n_rows; r += kThreads) {
-        if (p.row_seqs) {
-            p.row_seqs[r] = -1;
-        }
-        if (p.row_positions) {
-            p.row_positions[r] = -1;
-        }
-        if (p.row_slots) {
-            p.row_slots[r] = -1;
+    // ---- its share of the new entries of the table
+    if (enough) {
+        for (int64_t e = int64_t(blockIdx.x) * kThreads + tid; e < total[2]; e += int64_t(gridDim.x) * kThreads) {
+            const int chunk = chunk_of<kThreads>(s_grown, e);
+            int i = chunk * per, first = s_grown[chunk];
+            Request q = load_request(p, i, flags);
+            while (e >= first + q.grown) {
+                first += q.grown;
+                q = load_request(p, ++i, flags);
+            }
+            p.table[int64_t(q.row) * p.table_stride + q.held_pages + (e - first)] = p.free_pages[e];
         }
     }
-    atomicOr(&s_flags, flags);
-    __syncthreads();
-    if (threadIdx.x == 0) {
+    if (blockIdx.x == 0 && tid == 0) {
         if (p.q_starts) {
-            p.q_starts[p.n_seqs] = int(min(carry[0], int64_t(p.n_rows)));
+            p.q_starts[p.n_seqs] = int(min(total[0], int64_t(p.n_rows)));
         }
         if (p.page_starts) {
-            p.page_starts[p.n_seqs] = int(min(carry[1], int64_t(INT_MAX)));
+            p.page_starts[p.n_seqs] = int(min(total[1], int64_t(INT_MAX)));
         }
         if (p.status) {
             p.status[0] = enough ? int(total[2]) : 0;
-            p.status[1] = s_flags | (enough ? 0 : LLAISYS_PLAN_NO_PAGES) | (carry[0] > p.n_rows ? LLAISYS_PLAN_ROWS_DROPPED : 0);
+            p.status[1] = s_flags | (enough ? 0 : LLAISYS_PLAN_NO_PAGES) | (total[0] > p.n_rows ? LLAISYS_PLAN_ROWS_DROPPED : 0);
+        }
+    }
+
+    // ---- its share of the rows
+    if (p.row_seqs == nullptr && p.row_positions == nullptr && p.row_slots == nullptr) {
+        return;
+    }
+    const int live = int(min(total[0], int64_t(p.n_rows)));
+    for (int64_t r0 = (int64_t(blockIdx.x) * kThreads + tid) * kRowsAtOnce; r0 < p.n_rows; r0 += int64_t(gridDim.x) * kThreads * kRowsAtOnce) {
+        int seqs[kRowsAtOnce], positions[kRowsAtOnce];
+        int64_t slots[kRowsAtOnce];
+        const int lo = r0 < live ? chunk_of<kThreads>(s_rows, r0) : 0;
+        int i = lo * per;
+        int64_t start = s_rows[lo];
+        int grown = s_grown[lo];
+        Request q{};
+        int entry = -1, page = -1; // the entry of the table that `page` is from
+        bool loaded = false;
+#pragma unroll
+        for (int k = 0; k < kRowsAtOnce; ++k) {
+            const int64_t r = r0 + k;
+            seqs[k] = positions[k] = -1;
+            slots[k] = -1;
+            if (r >= live) {
+                continue;
+            }
+            while (!loaded || r >= start + q.fresh) {
+                if (loaded) {
+                    start += q.fresh;
+                    grown += q.grown;
+                    ++i;
+                }
+                q = load_request(p, i, flags);
+                loaded = true;
+                entry = -1;
+            }
+            const int pos = q.held + int(r - start);
+            seqs[k] = p.seq_ids ? p.seq_ids[i] : i;
+            positions[k] = pos;
+            if (p.row_slots != nullptr) {
+                const int e = p.page_shift >= 0 ? pos >> p.page_shift : pos / p.page_size;
+                if (e != entry) {
+                    entry = e;
+                    page = -1;
+                    if (q.row >= 0 && e < p.table_stride) {
+                        if (e < q.held_pages || p.free_pages == nullptr) {
+                            page = p.table[int64_t(q.row) * p.table_stride + e];
+                        } else if (enough && q.grown > 0) {
+                            page = p.free_pages[grown + e - q.held_pages]; // (its entry may be another CTA's to write)
+                        }
+                    }
+                }
+                slots[k] = page < 0 ? -1 : int64_t(page) * p.page_size + (pos - e * p.page_size);
+            }
+        }
+        if (p.rows_wide && r0 + kRowsAtOnce <= p.n_rows) {
+            if (p.row_seqs) {
+                *reinterpret_cast<int4 *>(p.row_seqs + r0) = make_int4(seqs[0], seqs[1], seqs[2], seqs[3]);
+            }
+            if (p.row_positions) {
+                *reinterpret_cast<int4 *>(p.row_positions + r0) = make_int4(positions[0], positions[1], positions[2], positions[3]);
+            }
+            if (p.row_slots) {
+                *reinterpret_cast<longlong2 *>(p.row_slots + r0) = make_longlong2(slots[0], slots[1]);
+                *reinterpret_cast<longlong2 *>(p.row_slots + r0 + 2) = make_longlong2(slots[2], slots[3]);
+            }
+            continue;
+        }
+#pragma unroll
+        for (int k = 0; k < kRowsAtOnce; ++k) {
+            if (r0 + k < p.n_rows) {
+                if (p.row_seqs) {
+                    p.row_seqs[r0 + k] = seqs[k];
+                }
+                if (p.row_positions) {
+                    p.row_positions[r0 + k] = positions[k];
+                }
+                if (p.row_slots) {
+                    p.row_slots[r0 + k] = slots[k];
+                }
+            }
         }
     }
 }
@@ -180,7 +266,23 @@ __global__ void __launch_bounds__(kThreads) paged_plan_kernel(PlanArgs p) {
 } // namespace
 
 void paged_plan(stream_t stream, const PlanArgs &args) {
-    paged_plan_kernel<<<1, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(args);
+    PlanArgs p = args;
+    p.page_shift = -1;
+    for (int s = 0; s < 31; ++s) {
+        p.page_shift = p.page_size == 1 << s ? s : p.page_shift;
+    }
+    p.rows_wide = aligned16(p.row_seqs) && aligned16(p.row_positions) && aligned16(p.row_slots);
+    // Up to 512 requests, four a thread, small CTAs: their sums take two barriers of four warps instead of 32. A turn of a CTA is four rows a thread.
+    auto start = [&](auto kernel, int threads) {
+        const int64_t turns = (std::max<int64_t>(p.n_rows, p.n_seqs) + threads * kRowsAtOnce - 1) / (threads * kRowsAtOnce);
+        const int64_t most = int64_t(device_sms()) * (threads == 1024 ? 2 : 4);
+        kernel<<<unsigned(std::max<int64_t>(1, std::min(turns, most))), threads, 0, static_cast<cudaStream_t>(stream)>>>(p);
+    };
+    if (p.n_seqs <= 512) {
+        start(paged_plan_kernel<128>, 128);
+    } else {
+        start(paged_plan_kernel<1024>, 1024);
+    }
     check_launch("paged_plan");
 }
 

@@ -381,12 +381,17 @@ class PagedKVCache:
             _addr(kv_lens_dev), n_seqs, total_q, max_q_len, max_kv_len, nh, scale, window, byref(gates), row_stride, stream))
 
 
-def paged_plan_dev(*, stream, device_id: int = 0, **fields) -> None:
+def paged_plan_dev(*, stream, held_dev, new_dev, n_seqs: int, page_size: int, n_rows: int, seq_ids_dev=None, free_pages_dev=None, n_free: int = 0,
+                   block_table_dev=None, table_rows: int = 0, table_stride: int = 0, q_starts_dev=None, kv_lens_dev=None, page_starts_dev=None,
+                   row_seqs_dev=None, row_positions_dev=None, row_slots_dev=None, status_dev=None, device_id: int = 0) -> None:
     """Index arrays of a step, slots and growth of the block table from the tokens that requests hold and bring, in one launch; fields of
     LlaisysPagedPlan (include/llaisys/paged_kv.h), buffers may be tensors."""
-    numbers = {"n_seqs", "page_size", "n_rows", "n_free", "table_rows", "table_stride"}
-    args = LlaisysPagedPlan(**{k: (v if k in numbers or v is None else _addr(v)) for k, v in fields.items()})
-    _check(LIB_LLAISYS.llaisysPagedPlanDev(int(DeviceType.NVIDIA), device_id, byref(args), stream))
+    args = LlaisysPagedPlan(_addr(seq_ids_dev), _addr(held_dev), _addr(new_dev), n_seqs, page_size, n_rows, _addr(free_pages_dev), n_free,
+                            _addr(block_table_dev), table_rows, table_stride, _addr(q_starts_dev), _addr(kv_lens_dev), _addr(page_starts_dev),
+                            _addr(row_seqs_dev), _addr(row_positions_dev), _addr(row_slots_dev), _addr(status_dev))
+    status = LIB_LLAISYS.llaisysPagedPlanDev(1, device_id, byref(args), stream)
+    if status:
+        _check(status)
 
 
 def linear_row_dev(dtype: DataType, out, x, gain, eps: float, weight, n: int, k: int, form: int, *, stream, device_id: int = 0) -> None:

@@ -7,10 +7,12 @@ from .libllaisys import LIB_LLAISYS
 
 def _addr(p) -> int | None:
     """Accepts an int address, a ctypes pointer, or anything with data_ptr() (Tensor, torch.Tensor)."""
-    if p is None:
-        return None
+    if p is None or type(p) is int:
+        return p
     if hasattr(p, "data_ptr"):
         p = p.data_ptr()
+        if type(p) is int:
+            return p
     if hasattr(p, "value"):
         p = p.value
     return int(p) if p is not None else None
