@@ -7,6 +7,7 @@
 //      4 (g / 2) + 2 j + g % 2, is word u = 2 s + j of the lane;
 //   V, output = P V (n = dim, k = token): a lane's scores of the two tiles are those of tokens 4 t ..+3, which makes them its A fragment of P
 //      as they are; word i of lane (g, t) holds the codes of those tokens for dim 8 i + g.
+// Codes are e4m3 numbers, or integers c kept as c + 128.
 // Word u of a lane lies at 16 (32 (u / 4) + lane) + 4 (u % 4); V follows K, and behind both lie the f32 scales of K and of V and 8 bytes of nothing.
 #pragma once
 
@@ -19,33 +20,7 @@ namespace llaisys::kernels {
 constexpr int kQuantTokens = 16;           // tokens of a block
 constexpr float kQuantFloor = 0x1p-100f;   // smallest scale an append writes
 
-__host__ __device__ __forceinline__ int quant_k_at(int token, int dim) {
-    const int u = 2 * (dim >> 4) + ((token >> 1) & 1), lane = 4 * (2 * (token >> 2) + (token & 1)) + ((dim >> 2) & 3);
-    return 16 * (32 * (u >> 2) + lane) + 4 * (u & 3) + (dim & 3);
-}
-__host__ __device__ __forceinline__ int quant_v_at(int token, int dim) { // from the first V code
-    const int u = dim >> 3, lane = 4 * (dim & 7) + (token >> 2);
-    return 16 * (32 * (u >> 2) + lane) + 4 * (u & 3) + (token & 3);
-}
 __host__ __device__ __forceinline__ int quant_scales_at(int d) { return 2 * kQuantTokens * d; }
-
-// Codes of a store: kF8 = e4m3, else integers c, kept as c + 128.
-template <bool kF8>
-__device__ __forceinline__ unsigned char quant_code(float x) {
-    if constexpr (kF8) {
-        return __nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3);
-    } else {
-        return static_cast<unsigned char>(128 + max(-127, min(127, __float2int_rn(x))));
-    }
-}
-template <bool kF8>
-__device__ __forceinline__ float quant_worth(unsigned char c) {
-    if constexpr (kF8) {
-        return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3)));
-    } else {
-        return float(int(c) - 128);
-    }
-}
 
 // Where a token lives. False (and flagged): not in the pool.
 __device__ __forceinline__ bool quant_tile_of(const QuantView &kv, int seq, int block, int32_t *error_flag, unsigned char *&tiles) {
