@@ -62,7 +62,8 @@ LLAISYS_API const char *llaisysGetLastError(void);
 #define LLAISYS_KERNEL_GATES_TC 9         /* gated attention of chunks on tcgen05 tensor cores                    */
 #define LLAISYS_KERNEL_LATENT_TC 10       /* attention over pages of latents (mixers.h) on tcgen05 tensor cores   */
 #define LLAISYS_KERNEL_EXPANDED_TC 11     /* chunk attention over keys and values made from latents, tcgen05      */
-#define LLAISYS_KERNEL_EIGHT_BIT 12       /* attention over pages held in 8 bits                                  */
+#define LLAISYS_KERNEL_EIGHT_BIT 12       /* attention over pages held in 8 bits, any call                        */
+#define LLAISYS_KERNEL_EIGHT_BIT_TC 13    /* the same of chunks on tcgen05 tensor cores                           */
 /* Kernel of the calling thread's most recent attention call: any cache, or llaisysSelfAttention. */
 LLAISYS_API int llaisysLastAttentionKernel(void);
 

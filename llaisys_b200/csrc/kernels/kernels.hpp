@@ -203,6 +203,10 @@ void attention_quant(stream_t stream, llaisysDataType_t dtype, const QuantView &
                      const AttnOut &out, const AttnScratch &scratch);
 // workspace of attention_quant on the current device, whatever the call (counters all zero between launches)
 void attention_quant_scratch(int32_t d, size_t *floats, size_t *counters);
+// The same for chunks on tcgen05: 16-bit activations, heads of 64 or 128. False: not covered, nothing queued.
+bool attention_quant_tc(stream_t stream, llaisysDataType_t dtype, const QuantView &kv, const AttnBatch &batch, const void *q, float scale,
+                        const AttnOut &out, const AttnScratch &scratch);
+void attention_quant_tc_scratch(int32_t d, size_t *floats, size_t *counters);
 // The index arrays of a step.
 void paged_plan(stream_t stream, const PlanArgs &args);
 void paged_gather(stream_t stream, size_t elem_size, const KVView &kv, int32_t seq_row, int32_t n_tokens,

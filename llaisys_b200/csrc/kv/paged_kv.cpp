@@ -167,6 +167,10 @@ PagedKV::PagedKV(const PagedKVConfig &cfg) : _cfg(cfg) {
         }
         if (quantized()) {
             kernels::attention_quant_scratch(int32_t(cfg.head_dim), &_partials_floats, &_counters_len);
+            size_t floats = 0, counters = 0;
+            kernels::attention_quant_tc_scratch(int32_t(cfg.head_dim), &floats, &counters);
+            _partials_floats = std::max(_partials_floats, floats);
+            _counters_len = std::max(_counters_len, counters);
         }
         if (_partials_floats != 0) {
             _partials = rt.allocateDeviceStorage(_partials_floats * sizeof(float));
@@ -545,9 +549,14 @@ int PagedKV::runQuant(size_t layer, const kernels::AttnBatch &b, const void *q, 
     KV_REQUIRE(opt.gates == nullptr && opt.fade_a == nullptr, LLAISYS_E_UNSUPPORTED,
                "paged attention: gated weights and distance penalties not for a cache held in 8 bits");
 #ifdef ENABLE_NVIDIA_API
-    kernels::attention_quant(stream, _cfg.dtype, quantView(layer), b, q, scale, o, scratch());
-    noteAttentionKernel(LLAISYS_KERNEL_EIGHT_BIT);
-    return LLAISYS_KERNEL_EIGHT_BIT;
+    const kernels::QuantView v = quantView(layer);
+    int used = LLAISYS_KERNEL_EIGHT_BIT_TC;
+    if (!kernels::attention_quant_tc(stream, _cfg.dtype, v, b, q, scale, o, scratch())) {
+        kernels::attention_quant(stream, _cfg.dtype, v, b, q, scale, o, scratch());
+        used = LLAISYS_KERNEL_EIGHT_BIT;
+    }
+    noteAttentionKernel(used);
+    return used;
 #else
     (void)layer, (void)b, (void)q, (void)scale, (void)o, (void)stream;
     fail(LLAISYS_E_UNSUPPORTED, "this build has no NVIDIA backend");

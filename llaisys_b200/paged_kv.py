@@ -36,6 +36,7 @@ class Kernel(IntEnum):
     LATENT_TC = 10
     EXPANDED_TC = 11
     EIGHT_BIT = 12
+    EIGHT_BIT_TC = 13
 
 
 def last_attention_kernel() -> Kernel:
