@@ -30,7 +30,7 @@ namespace llaisys::kernels {
 
 namespace {
 
-constexpr int kSoftmaxThreads = 128, kMmaWarp = 8, kWidenWarp = 10, kWidenWarps = 4, kThreads = 512;
+constexpr int kSoftmaxThreads = 128, kMmaWarp = 8, kWidenWarp = 10, kWidenWarps = 4, kGuideWarp = kWidenWarp + kWidenWarps, kThreads = 512;
 // Registers a thread: 512 x 128 at launch, then 256 softmax threads take 200 and the other eight warps (two of them idle) keep 56. (Fourteen warps
 // would be launched with 128 as well: a quarter of the SM holds four of them.)
 constexpr int kSoftmaxRegs = 200, kOtherRegs = 56;
@@ -40,6 +40,8 @@ static_assert(sizeof(Place) <= kPlaceInts * sizeof(int), "a warp's words");
 constexpr int kErrTimeout = 8;
 constexpr float kRescaleThreshold = 8.f; // log2 units
 constexpr float kShift = 7.f;            // weights are 2^7 times what they stand for: at most 2^15 with a maximum that lags by the threshold
+constexpr int kFeedSlots = 4;            // blocks whose tiles the guide has found ahead of the operand warps
+constexpr int kPlaces = 11;              // warps that keep a place on the line: all but the operand warps and the last one
 constexpr int kScaleSlots = 4;           // blocks whose scales are kept: a block's slot is written again when its turn has passed twice over
 constexpr float kMergeCostBlocks = 1.5f;
 constexpr int kMergeCost = 5;
@@ -48,12 +50,12 @@ template <int D>
 struct Shape {
     static constexpr int kStages = 5, kStageBytes = kKeys * D * 2;
     static constexpr int kKPiece = kKeys * 128, kVPiece = D * 128, kQPiece = kHalf * 128, kQBytes = kHalf * D * 2;
-    static constexpr int kTmemCols = D == 128 ? 512 : 512, kColS = 0, kColO = 2 * kKeys; // scores of half h at 128 h, accumulators behind them
+    static constexpr int kTmemCols = 512, kColS = 0, kColO = 2 * kKeys; // scores of half h at 128 h, accumulators behind them
     static constexpr int kPartialFloats = kHalf * D + 2 * kHalf;
-    static constexpr int kBars = 2 * kStages + 14;
+    static constexpr int kBars = 2 * kStages + 14 + 2 * kFeedSlots;
     static constexpr size_t kScales = 2 * size_t(kQBytes) + kStages * size_t(kStageBytes), kFactors = kScales + kScaleSlots * kPagesPerBlock * 16;
     static constexpr size_t kBarsAt = kFactors + 2 * kRows, kSched = kBarsAt + kBars * 8 + 8;
-    static constexpr size_t kBytes = kSched + (kSchedInts + kWarpsOfCta * kPlaceInts) * sizeof(int);
+    static constexpr size_t kFeed = kSched + (kSchedInts + kPlaces * kPlaceInts) * sizeof(int), kBytes = kFeed + kFeedSlots * kPagesPerBlock * 12;
     static_assert(kBytes <= 227 * 1024, "shared memory of an SM");
 };
 
@@ -92,6 +94,12 @@ __device__ __forceinline__ uint2 widen(uint32_t w) {
     }
 }
 __device__ __forceinline__ void sts64(uint32_t addr, uint2 v) { asm volatile("st.shared.v2.u32 [%0], {%1, %2};\n" ::"r"(addr), "r"(v.x), "r"(v.y) : "memory"); }
+// 8 columns of this thread's TMEM lane, raw words.
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&w)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"r"(taddr), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+                 "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+}
 __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t *>(&h);
@@ -119,7 +127,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_quant_tc_kernel(QuantCh
         kBarDrain = kBarTurn + 2,       // [2] MMA (commit) -> the issuer itself: everything it issued has finished
         kBarP = kBarDrain + 2,          // [2][2] softmax (128) -> MMA: this part of P is in tensor memory (and the accumulator rescaled)
         kBarQ = kBarP + 4,              // [2] softmax (128) -> MMA: the next fragment's Q rows are in shared memory
-        kNumBars = kBarQ + 2
+        kBarFound = kBarQ + 2,               // [kFeedSlots] guide -> operand warps: the tiles of a block are known
+        kBarRead = kBarFound + kFeedSlots,   // [kFeedSlots] operand warps (one arrival each) -> guide: and have been read
+        kNumBars = kBarRead + kFeedSlots
     };
     static_assert(kNumBars == S::kBars, "barriers");
     extern __shared__ __align__(1024) unsigned char smem_raw[];
@@ -264,7 +274,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_quant_tc_kernel(QuantCh
     // ---- set-up: barriers, TMEM ----------------------------------------------------------------------------------
     if (tid == 0) {
         for (int i = 0; i < kNumBars; ++i) {
-            mbar_init(bars_u32 + i * 8, i >= kBarP ? kSoftmaxThreads : i >= kBarEmpty && i < kBarS ? 2 : i < kBarEmpty ? kWidenWarps : 1);
+            mbar_init(bars_u32 + i * 8, i >= kBarRead || i < kBarEmpty ? kWidenWarps : i >= kBarFound ? 1 : i >= kBarP ? kSoftmaxThreads : i < kBarS ? 2 : 1);
         }
         *s_abort = 0;
         mbar_init_fence();
@@ -296,7 +306,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_quant_tc_kernel(QuantCh
     };
     // A warp's place on the line waits in shared memory while its blocks run: a register that is spilled there is fetched from L2 (the
     // operands leave no L1), and a dozen such loads per block cost as much as the block.
-    Place *place = reinterpret_cast<Place *>(s_sched + kSchedInts + warp * kPlaceInts);
+    Place *place = reinterpret_cast<Place *>(s_sched + kSchedInts + min(warp < kWidenWarp ? warp : warp - kWidenWarps, kPlaces - 1) * kPlaceInts);
     auto keep_place = [&](const Walker &w, const Fragment &f, int pos) {
         __syncwarp();
         if (lane == 0) {
@@ -306,7 +316,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_quant_tc_kernel(QuantCh
         }
         __syncwarp();
     };
-    keep_place(walker, Fragment{}, piece_begin);
+    if (warp < kWidenWarp || warp == kGuideWarp) {
+        keep_place(walker, Fragment{}, piece_begin);
+    }
     // The next fragment of the piece, in this warp's place.
     auto next_fragment = [&](Walker &w, Fragment &f) {
         int pos = place->pos;
@@ -319,8 +331,79 @@ __global__ void __launch_bounds__(kThreads, 1) attention_quant_tc_kernel(QuantCh
     // (setmaxnreg inside each branch: where they met again the compiler would keep to the smaller count)
     if (warp >= kMmaWarp) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kOtherRegs));
-        if (warp >= kWidenWarp + kWidenWarps) {
-            // (idle: its registers are the softmax's)
+        // What the guide tells the operand warps of a block of 16 keys: its tile's place in the pool (kNone: there is none, kEnd: no more blocks) and scales.
+        struct Found {
+            int place;
+            float s_k, s_v;
+        };
+        constexpr int kNone = -1, kEnd = -2;
+        Found *s_feed = reinterpret_cast<Found *>(base + S::kFeed); // [kFeedSlots][kPagesPerBlock]
+        if (warp == kGuideWarp) {
+            // ================================ guide: where the blocks' tiles are =====================================
+            // Pages come 4 blocks (32 blocks of 16 keys, a lane each) at a time, the group behind a group early. Behind a tile's last block its last
+            // block comes again: hidden keys have weight 0, and what they are multiplied by is then always of this sequence.
+            constexpr int kGroup = 32 / kPagesPerBlock;
+            uint32_t told = 0; // blocks
+            auto tell = [&](const Found &found, int from) { // lanes from, ..., from + 7
+                const int at = told % kFeedSlots;
+                if (told >= kFeedSlots && !__all_sync(0xffffffffu, wait(kBarRead + at, told / kFeedSlots - 1))) {
+                    return false;
+                }
+                if (lane >= from && lane < from + kPagesPerBlock) {
+                    s_feed[at * kPagesPerBlock + lane - from] = found;
+                }
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(bar(kBarFound + at));
+                }
+                ++told;
+                return true;
+            };
+            bool alive = true;
+            while (alive) {
+                Fragment f;
+                Walker w;
+                if (!next_fragment(w, f)) {
+                    break;
+                }
+                const int n = f.b1 - f.b0, seq = p.seq_ids[f.a];
+                const int last = (min(tile_kv_hi(w.g, f.qb), min(max(p.kv_lens[f.a], 0), p.table_stride * kPage)) + kPage - 1) / kPage - 1;
+                const bool known = seq >= 0 && seq < p.kv.table_rows;
+                if (!known) {
+                    atomicOr(p.error_flag, kErrBadSeq);
+                }
+                const int32_t *table = p.kv.block_table + (long long)(known ? seq : 0) * p.kv.table_stride;
+                auto find = [&](int blk0) {
+                    Found found{kNone, 0.f, 0.f};
+                    const int b = blk0 + lane / kPagesPerBlock;
+                    const int at = min((kWin && b >= w.g.kept_blocks ? b + f.gap : b) * kPagesPerBlock + lane % kPagesPerBlock, last);
+                    if (at >= 0 && known) { // (else: no token at all, no sequence)
+                        const int entry = p.kv.blocks_per_page == 1 ? at : at / p.kv.blocks_per_page, page = table[entry];
+                        if (page < 0 || page >= p.kv.num_pages) {
+                            atomicOr(p.error_flag, kErrBadPage);
+                        } else {
+                            found.place = (page * p.kv.blocks_per_page + at - entry * p.kv.blocks_per_page) * p.kv.nkvh + f.kvh;
+                            const float2 scales = __ldcg(reinterpret_cast<const float2 *>(p.kv.base + (long long)found.place * p.kv.tile_bytes + quant_scales_at(D)));
+                            found.s_k = scales.x;
+                            found.s_v = scales.y;
+                        }
+                    }
+                    return found;
+                };
+                Found group = find(f.b0), next_group = find(f.b0 + kGroup);
+                for (int i = 0; i < n && alive; ++i) {
+                    if (i > 0 && i % kGroup == 0) {
+                        group = next_group;
+                        next_group = find(f.b0 + i + kGroup);
+                    }
+                    alive = tell(group, i % kGroup * kPagesPerBlock);
+                }
+            }
+            if (alive) {
+                tell(Found{kEnd, 0.f, 0.f}, 0);
+            }
+        } else if (warp > kGuideWarp) {
+            // (idle)
         } else if (warp >= kWidenWarp) {
             // ================================ operands: codes to f16 =================================================
             constexpr int kVecs = D / 32;
@@ -332,82 +415,29 @@ __global__ void __launch_bounds__(kThreads, 1) attention_quant_tc_kernel(QuantCh
                                            ((((odd << 1) | (t >> 1)) ^ ((((g >> 1) & 1) << 2) | odd)) << 4) + (t & 1) * 8);
             // V, word k of vector v of the block `other` (0: a, 1: the one 32 keys on): dim 32 v + 8 k + g, tokens 4 t; lanes of odd g begin with the other block
             const uint32_t v_at = uint32_t((block_a >> 2) * kVPiece + g * 128 + (((((block_a & 3) << 1) | (t >> 1)) ^ (odd << 2) ^ g) << 4) + (t & 1) * 8);
-            // The two blocks' tiles in each block of the walk: pages come 4 blocks (32 blocks of 16) at a time, the group behind a group early. Behind a
-            // tile's last block its last block comes again: hidden keys have weight 0, and what they are multiplied by is then always of this sequence.
-            const int32_t *table = nullptr; // of the fragment's sequence
-            int n = 0, i = 0, b0 = 0, kept = 0, gap = 0, last = -1, kvh = 0, group = -1, next_group = -1;
-            auto load_group = [&](int blk0) {
-                const int b = blk0 + lane / kPagesPerBlock;
-                const int at = min((kWin && b >= kept ? b + gap : b) * kPagesPerBlock + lane % kPagesPerBlock, last);
-                if (at < 0 || table == nullptr) { // (no token at all, no sequence)
-                    return -1;
-                }
-                const int entry = p.kv.blocks_per_page == 1 ? at : at / p.kv.blocks_per_page;
-                const int page = table[entry];
-                if (page < 0 || page >= p.kv.num_pages) {
-                    atomicOr(p.error_flag, kErrBadPage);
-                    return -1;
-                }
-                return (page * p.kv.blocks_per_page + at - entry * p.kv.blocks_per_page) * p.kv.nkvh + kvh;
-            };
-            constexpr int kGroup = 32 / kPagesPerBlock;
-            const unsigned char *tiles[2] = {nullptr, nullptr};
-            bool more = true;
+            // The registers of these warps hold one UNIT of codes, 16 words a lane: K of one block of 16 keys, or the low or high half of the dims of V of
+            // both. As soon as a word is read its register is asked to bring the next unit's. (Two units would be a stage, and spill: what is spilled
+            // here comes back from L2, the operands leave no L1.)
+            int tiles[2] = {kNone, kNone}; // places of the two tiles of the units that are asked for
+            uint32_t heard = 0;            // blocks
+            bool more = true, ok = true;
             auto step = [&]() { // to the next block: its tiles
-                if (i + 1 < n) {
-                    if (++i % kGroup == 0) {
-                        group = next_group;
-                        next_group = load_group(b0 + i + kGroup);
-                    }
-                } else {
-                    Fragment f;
-                    Walker w;
-                    if (!next_fragment(w, f)) {
-                        more = false;
-                        return;
-                    }
-                    n = f.b1 - f.b0;
-                    i = 0;
-                    b0 = f.b0;
-                    kvh = f.kvh;
-                    if constexpr (kWin) {
-                        kept = w.g.kept_blocks;
-                        gap = f.gap;
-                    }
-                    last = (min(tile_kv_hi(w.g, f.qb), min(max(p.kv_lens[f.a], 0), p.table_stride * kPage)) + kPage - 1) / kPage - 1;
-                    const int seq = p.seq_ids[f.a];
-                    table = nullptr;
-                    if (seq >= 0 && seq < p.kv.table_rows) {
-                        table = p.kv.block_table + (long long)seq * p.kv.table_stride;
-                    } else {
-                        atomicOr(p.error_flag, kErrBadSeq);
-                    }
-                    group = load_group(b0);
-                    next_group = load_group(b0 + kGroup);
-                }
-#pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    const int place = __shfl_sync(0xffffffffu, group, i % kGroup * kPagesPerBlock + block_a + 2 * b);
-                    tiles[b] = place < 0 ? nullptr : p.kv.base + (long long)place * tile_bytes;
-                }
+                const int at = heard % kFeedSlots;
+                ok = __all_sync(0xffffffffu, wait(kBarFound + at, heard / kFeedSlots)) && ok;
+                tiles[0] = s_feed[at * kPagesPerBlock + block_a].place;
+                tiles[1] = s_feed[at * kPagesPerBlock + block_a + 2].place;
+                more = ok && tiles[0] != kEnd;
             };
-            uint4 raw[2][kVecs];
-            auto fetch = [&](int b, int v, bool is_v) {
-                raw[b][v] = tiles[b] != nullptr ? __ldcg(reinterpret_cast<const uint4 *>(tiles[b] + (is_v ? kQuantTokens * D : 0)) + 32 * v + lane)
-                            : kF8               ? make_uint4(0, 0, 0, 0)
-                                                : make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
+            constexpr int kHalfVecs = kVecs / 2; // 16-byte loads of a unit of V from either tile
+            uint4 raw[2 * kHalfVecs];
+            const uint4 none = kF8 ? make_uint4(0, 0, 0, 0) : make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
+            auto code_at = [&](int b, int at) { // 16 bytes of tile b
+                return tiles[b] >= 0 ? __ldcg(reinterpret_cast<const uint4 *>(p.kv.base + (long long)tiles[b] * tile_bytes) + at + lane) : none;
             };
-            float2 scales = make_float2(0.f, 0.f); // of tile `lane`, lanes 0 and 1
-            auto fetch_scales = [&]() {
-                const unsigned char *tile = lane == 0 ? tiles[0] : tiles[1];
-                scales = make_float2(0.f, 0.f);
-                if (lane < 2 && tile != nullptr) {
-                    scales = __ldcg(reinterpret_cast<const float2 *>(tile + quant_scales_at(D)));
-                }
-            };
+            auto fetch_k = [&](int b, int v) { raw[v] = code_at(b, 32 * v); };
+            auto fetch_v = [&](int half, int k) { raw[k] = code_at(k / kHalfVecs, kQuantTokens * D / 16 + 32 * (half * kHalfVecs + k % kHalfVecs)); };
             int stage = 0;
-            uint32_t turn = 0, blocks = 0;
-            bool ok = true;
+            uint32_t turn = 0;
             auto take_stage = [&]() {
                 if (turn > 0) {
                     ok = __all_sync(0xffffffffu, wait(kBarEmpty + stage, turn - 1)) && ok;
@@ -425,62 +455,75 @@ __global__ void __launch_bounds__(kThreads, 1) attention_quant_tc_kernel(QuantCh
                     ++turn;
                 }
             };
+            // K of block b of the two, word j of vector v
+            auto put_k = [&](uint32_t to, int b, int v, const uint4 &x) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t u = j == 0 ? (odd ? x.z : x.x) : j == 1 ? (odd ? x.w : x.y) : j == 2 ? (odd ? x.x : x.z) : (odd ? x.y : x.w);
+                    // (bits 4 to 6 of a row's place are swizzled: 32 dims are bit 6, 16 dims bit 5, two tokens bit 5 and a row of 256 bytes on)
+                    sts64(to + (v >> 1) * kKPiece + b * 32 * 128 + (j & 1) * 256 + (k_at ^ uint32_t(((v & 1) << 6) | (((j >> 1) ^ (j & 1)) << 5))),
+                          widen<kF8>(u));
+                }
+            };
             step();
-            fetch_scales();
 #pragma unroll
             for (int v = 0; v < kVecs; ++v) {
-                fetch(0, v, false);
-                fetch(1, v, false);
+                fetch_k(0, v);
             }
             while (more && ok) {
-                // ---- K of the block; its V is asked for word by word
+                // ---- K of the block
                 uint32_t to = take_stage();
                 if (!ok) {
                     break;
                 }
                 if (lane < 2) {
-                    const float s_v = scales.y < kQuantFloor ? kQuantFloor : scales.y; // (a block never written to; NaN stays)
-                    s_scales[(blocks % kScaleSlots) * kPagesPerBlock + block_a + 2 * lane] = make_float4(scales.x, fast_log2(s_v), 1.f / s_v, 0.f);
+                    const int b = heard % kFeedSlots * kPagesPerBlock + block_a + 2 * lane;
+                    const float s_v = s_feed[b].s_v < kQuantFloor ? kQuantFloor : s_feed[b].s_v; // (a block never written to; NaN stays)
+                    s_scales[heard % kScaleSlots * kPagesPerBlock + block_a + 2 * lane] = make_float4(s_feed[b].s_k, fast_log2(s_v), 1.f / s_v, 0.f);
                 }
-                ++blocks;
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(bar(kBarRead + heard % kFeedSlots));
+                }
+                ++heard;
 #pragma unroll
                 for (int v = 0; v < kVecs; ++v) {
+                    put_k(to, 0, v, raw[v]);
+                    fetch_k(1, v);
+                }
 #pragma unroll
-                    for (int b = 0; b < 2; ++b) {
-                        const uint4 x = raw[b][v];
-                        const uint32_t u[4] = {odd ? x.z : x.x, odd ? x.w : x.y, odd ? x.x : x.z, odd ? x.y : x.w};
-                        fetch(b, v, true);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            // (bits 4 to 6 of a row's place are swizzled: 32 dims are bit 6, 16 dims bit 5, two tokens bit 5 and a row of 256 bytes on)
-                            sts64(to + (v >> 1) * kKPiece + b * 32 * 128 + (j & 1) * 256 + (k_at ^ uint32_t(((v & 1) << 6) | (((j >> 1) ^ (j & 1)) << 5))),
-                                  widen<kF8>(u[j]));
-                        }
-                    }
+                for (int v = 0; v < kVecs; ++v) {
+                    put_k(to, 1, v, raw[v]);
+                    fetch_v(0, v);
                 }
                 give_stage();
-                // ---- V of the block; K of the next one is asked for
+                // ---- V of the block
                 to = take_stage();
                 if (!ok) {
                     break;
                 }
-                step();
-                if (more) {
-                    fetch_scales();
-                }
 #pragma unroll
-                for (int v = 0; v < kVecs; ++v) {
-                    const uint4 a = raw[0][v], c = raw[1][v];
-                    const uint32_t first[4] = {odd ? c.x : a.x, odd ? c.y : a.y, odd ? c.z : a.z, odd ? c.w : a.w};
-                    const uint32_t second[4] = {odd ? a.x : c.x, odd ? a.y : c.y, odd ? a.z : c.z, odd ? a.w : c.w};
-                    if (more) {
-                        fetch(0, v, false);
-                        fetch(1, v, false);
+                for (int half = 0; half < 2; ++half) {
+                    if (half == 1) {
+                        step(); // (V is asked for; K of the next block comes next)
                     }
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        sts64(to + (32 * v + 8 * j) * 128 + v_at, widen<kF8>(first[j]));
-                        sts64(to + (32 * v + 8 * j) * 128 + (v_at ^ 64u), widen<kF8>(second[j]));
+                    for (int v = 0; v < kHalfVecs; ++v) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const uint4 &a = raw[v], &c = raw[kHalfVecs + v];
+                            const uint32_t x = j == 0 ? a.x : j == 1 ? a.y : j == 2 ? a.z : a.w, y = j == 0 ? c.x : j == 1 ? c.y : j == 2 ? c.z : c.w;
+                            const uint32_t row = to + (32 * (half * kHalfVecs + v) + 8 * j) * 128;
+                            sts64(row + v_at, widen<kF8>(odd ? y : x));
+                            sts64(row + (v_at ^ 64u), widen<kF8>(odd ? x : y));
+                        }
+                        if (half == 0) {
+                            fetch_v(1, v);
+                            fetch_v(1, kHalfVecs + v);
+                        } else if (more) {
+                            fetch_k(0, v);
+                            fetch_k(0, kHalfVecs + v);
+                        }
                     }
                 }
                 give_stage();
@@ -677,9 +720,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_quant_tc_kernel(QuantCh
             Fragment f = place->f;
             SeqGeom g = place->w.g;
             const int n = f.b1 - f.b0;
-            const int x = f.qb * kRows + h * kHalf + row, t = per_group(x), head = f.kvh * p.group + (x - t * p.group);
             // (the line counts a chunk that is longer than what the sequence holds as if it held it; here its first queries see nothing)
-            const int tokens = min(max(p.kv_lens[f.a], 0), p.table_stride * kPage), last_visible = t + tokens - g.q_len; // keys j <= last_visible take part
+            const int tokens = min(max(p.kv_lens[f.a], 0), p.table_stride * kPage);
+            const int last_visible = per_group(f.qb * kRows + h * kHalf + row) + tokens - g.q_len; // keys j <= last_visible take part
             const int n_seen = min(last_visible + 1, tokens);
             float m_used = -INFINITY, l = 0.f;
             named_barrier_sync(1 + h, kSoftmaxThreads); // the factors of all rows are there
@@ -733,20 +776,16 @@ __global__ void __launch_bounds__(kThreads, 1) attention_quant_tc_kernel(QuantCh
                         }
                     }
                 }
-                // row maximum as eight independent chains
-                float mx8[8];
-#pragma unroll
-                for (int u = 0; u < 8; ++u) {
-                    mx8[u] = -INFINITY;
-                }
+                // row maximum as four independent chains
+                float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                 for (int c = 0; c < kKeys / 32; ++c) {
 #pragma unroll
                     for (int k = 0; k < 16; ++k) {
-                        mx8[k & 7] = max3(mx8[k & 7], __uint_as_float(sr[c][k]), __uint_as_float(sr[c][k + 16]));
+                        mx4[k & 3] = max3(mx4[k & 3], __uint_as_float(sr[c][k]), __uint_as_float(sr[c][k + 16]));
                     }
                 }
-                const float mx = max3(max3(mx8[0], mx8[1], mx8[2]), max3(mx8[3], mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7]));
+                const float mx = fmaxf(max3(mx4[0], mx4[1], mx4[2]), mx4[3]);
                 // The running max only moves when it grew by more than 2^8: P and the row sum both use m_used, so the result is exact
                 // either way, and O is rescaled rarely. (The scores' arrival says that the product of the block before is done.)
                 float alpha = 1.f;
@@ -770,26 +809,23 @@ __global__ void __launch_bounds__(kThreads, 1) attention_quant_tc_kernel(QuantCh
                 }
                 const float neg_m = m_used == -INFINITY ? 0.f : kShift - m_used;
 #pragma unroll
-                for (int c = 0; c < kKeys / 32; ++c) { // 32 keys = 16 columns of packed pairs over the scores
-                    float packed[16];
+                for (int b = 0; b < kPagesPerBlock; ++b) { // 16 keys = 8 columns of packed pairs over the scores
+                    uint32_t packed[8];
+                    float l0 = 0.f, l1 = 0.f;
 #pragma unroll
-                    for (int b = 0; b < 2; ++b) {
-                        float l0 = 0.f, l1 = 0.f;
-#pragma unroll
-                        for (int k = 16 * b; k < 16 * b + 16; k += 2) {
-                            float x0 = __uint_as_float(sr[c][k]), x1 = __uint_as_float(sr[c][k + 1]);
-                            add2(x0, x1, neg_m, neg_m);
-                            const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
-                            add2(l0, l1, p0, p1);
-                            packed[k >> 1] = __uint_as_float(pack_half2(p0, p1));
-                        }
-                        l = fmaf(l0 + l1, block_scales[2 * c + b].z, l);
+                    for (int k = 0; k < 16; k += 2) {
+                        float x0 = __uint_as_float(sr[b >> 1][(b & 1) * 16 + k]), x1 = __uint_as_float(sr[b >> 1][(b & 1) * 16 + k + 1]);
+                        add2(x0, x1, neg_m, neg_m);
+                        const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
+                        add2(l0, l1, p0, p1);
+                        packed[k >> 1] = pack_half2(p0, p1);
                     }
-                    tmem_st16(tmem_s + c * 16, packed);
-                    if (c & 1) {
+                    l = fmaf(l0 + l1, block_scales[b].z, l);
+                    tmem_st8(tmem_s + b * 8, packed);
+                    if ((b & 3) == 3) {
                         tmem_wait_st();
                         tc_fence_before();
-                        mbar_arrive(bar(kBarP + h * 2 + (c >> 1)));
+                        mbar_arrive(bar(kBarP + h * 2 + (b >> 2)));
                     }
                 }
             }
@@ -797,6 +833,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_quant_tc_kernel(QuantCh
             asm volatile("" ::: "memory");
             f = place->f;
             g = place->w.g;
+            const int x = f.qb * kRows + h * kHalf + row, t = per_group(x), head = f.kvh * p.group + (x - t * p.group);
             const int last_load = 2 * (done + n) - 1; // V of the last block
             done += n;
             move_on();
