@@ -24,6 +24,7 @@
 #include "tcgen05_utils.cuh"
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 namespace llaisys::kernels {
@@ -478,8 +479,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_quant_tc_kernel(QuantCh
                 }
                 if (lane < 2) {
                     const int b = heard % kFeedSlots * kPagesPerBlock + block_a + 2 * lane;
-                    const float s_v = s_feed[b].s_v < kQuantFloor ? kQuantFloor : s_feed[b].s_v; // (a block never written to; NaN stays)
-                    s_scales[heard % kScaleSlots * kPagesPerBlock + block_a + 2 * lane] = make_float4(s_feed[b].s_k, fast_log2(s_v), 1.f / s_v, 0.f);
+                    // (a block never written to has no scale; the NaN of a lost one is in the logarithm, and so in the weights of whoever sees it, and not in
+                    // what the sums of all others are multiplied by)
+                    const float s_v = s_feed[b].s_v < kQuantFloor ? kQuantFloor : s_feed[b].s_v;
+                    s_scales[heard % kScaleSlots * kPagesPerBlock + block_a + 2 * lane] = make_float4(s_feed[b].s_k, fast_log2(s_v), isnan(s_v) ? 0.f : 1.f / s_v, 0.f);
                 }
                 __syncwarp();
                 if (lane == 0) {
@@ -982,6 +985,20 @@ __global__ void __launch_bounds__(kThreads, 1) attention_quant_tc_kernel(QuantCh
     }
 }
 
+// Whether this kernel is the faster one for a call, of what the host knows of it (sums and the longest lengths). Microseconds on an SM; the
+// other kernel works on 16 rows x 16 keys at a time (0.23 a CTA of two on an SM, a tile of rows costs about 20 of them besides), this one on 256 x
+// 128 (3.5, pieces of no less than sqrt(1.5 longest tile) blocks). Measured, 12 / 2 heads of 128, us there and here: 64 chunks of 8 behind 4000
+// tokens 90 and 109, of 16 162 and 110; 8 of 16 behind 4000 35 and 40, of 32 53 and 44; one of 64 behind 300 15 and 22; 32 / 8 heads, 64 chunks of 4
+// behind 300 23 and 64, of 16 72 and 66.
+bool wide_tiles_pay(const AttnBatch &batch, int nkvh, int group) {
+    const double sms = device_sms(), rows = double(batch.total_q) * group;
+    const double seen = batch.window > 0 ? std::min(double(batch.max_kv_len), double(batch.window) + batch.keep_first + 256) : double(batch.max_kv_len);
+    const double small = (0.5 * batch.n_seqs + rows / 16) * nkvh, large = (batch.n_seqs + rows / 256) * nkvh, longest = std::ceil(seen / kKeys);
+    const double there = 8 + 0.23 * std::max(small * (seen / 16 + 20) / (2 * sms), 16.0);
+    const double here = 7 + 3.5 * std::max(large * (longest + 2) / sms, std::min(longest, std::max(3.0, std::sqrt(1.5 * longest))));
+    return here < there;
+}
+
 } // namespace
 
 void attention_quant_tc_scratch(int32_t d, size_t *floats, size_t *counters) {
@@ -996,7 +1013,7 @@ bool attention_quant_tc(stream_t stream, llaisysDataType_t dtype, const QuantVie
     const int group = batch.nh / kv.nkvh;
     if (!(bf16 || dtype == LLAISYS_DTYPE_F16) || (kv.d != 64 && kv.d != 128) || batch.q_starts == nullptr || out.out == nullptr || out.part != nullptr ||
         group > 32 || int64_t(batch.total_q) * group >= int64_t(1) << 26 || !aligned16(q) || !aligned16(out.out) || out.row_stride % 8 != 0 ||
-        int64_t(kv.table_stride) * kv.blocks_per_page * kPage > 0x7fffffff) {
+        int64_t(kv.table_stride) * kv.blocks_per_page * kPage > 0x7fffffff || !wide_tiles_pay(batch, kv.nkvh, group)) {
         return false;
     }
     size_t floats, counters;

@@ -34,7 +34,7 @@ __device__ __forceinline__ SeqGeom seq_geom(const P &p, int a) {
     } else {
         g.q_start = p.q_starts[a];
         g.q_len = p.q_starts[a + 1] - g.q_start;
-        g.kv_len = min(max(p.kv_lens[a], g.q_len), p.table_stride * kPage);
+        g.kv_len = P::kQueriesMayLead ? max(min(p.kv_lens[a], p.table_stride * kPage), g.q_len) : min(max(p.kv_lens[a], g.q_len), p.table_stride * kPage);
     }
     g.q_len = min(g.q_len, g.kv_len); // (a chunk longer than the tables can hold: flagged elsewhere, never off the end here)
     g.off = g.kv_len - g.q_len;

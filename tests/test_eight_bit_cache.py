@@ -325,6 +325,61 @@ def test_windows_factors_and_strides(cuda_device, window, keep, dtype, store, d)
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("store", ["i8", "f8"])
+@pytest.mark.parametrize("dtype,nh,nkvh,d,page", [("bf16", 12, 2, 128, 16), ("f16", 32, 8, 64, 32), ("bf16", 16, 1, 128, 64), ("f16", 8, 8, 128, 16),
+                                                  ("bf16", 24, 1, 64, 16)])
+def test_long_chunks(cuda_device, store, dtype, nh, nkvh, d, page):
+    f = Filled([4, 900, 300, 513, 1029, 2050], nkvh, d, dtype, store, page)
+    parts = [(3, 513), (0, 3), (5, 700), (1, 900), (4, 1), (2, 299)]
+    f.check_attention(parts, nh, chunks=True)
+    assert f.cache.last_kernel() == llaisys.Kernel.EIGHT_BIT_TC
+    factor = torch.randn(2416, nh, generator=torch.Generator().manual_seed(3))
+    for window, keep in ((1, 0), (100, 17), (600, 300)):
+        f.check_attention(parts, nh, window=window, keep=keep, factor=factor, stride=nh * d + 16, chunks=True)
+        assert f.cache.last_kernel() == llaisys.Kernel.EIGHT_BIT_TC
+    f.cache.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("window", [0, 40])
+def test_long_chunks_longer_than_their_sequences_and_lost_blocks(cuda_device, window):
+    nh, d = 8, 128
+    f = Filled([700, 260, 1], 2, d, "bf16", "i8", extra=16)
+    bad = f.rows(1)
+    bad[0, 0, 3] = torch.inf
+    f.append([(0, 400, 1)], bad, f.rows(1))
+    f.append([(1, 17, 1)], f.rows(1), bad)
+    q = torch.randn(2700, nh, d, generator=torch.Generator().manual_seed(5)).bfloat16()
+    starts, lens = [0, 900, 1800, 2600, 2600], [700, 260, 1, 0]
+    out = torch.full((2700, nh, d), 9.0, dtype=torch.bfloat16, device="cuda")
+    qd = q.cuda()
+    ids = i32([*f.seqs, 0])
+    f.cache.attention_dev(0, out, qd, ids, i32(starts), i32(lens), n_seqs=4, total_q=2600, max_q_len=900, max_kv_len=700, nh=nh, scale=-0.05,
+                          stream=stream(), window=window)
+    assert f.cache.last_kernel() == llaisys.Kernel.EIGHT_BIT_TC
+    got = out.cpu().double()
+    assert (got[2600:] == 9).all()
+    for i in range(3):
+        n, at = starts[i + 1] - starts[i], starts[i]
+        k, v = (torch.from_numpy(x.worth()).double() for x in (f.k[i], f.v[i]))
+        lead = n - lens[i]  # queries in front of the first token
+        assert (got[at:at + lead] == 0).all()
+        want, top, big = attention_f64(q[at + lead:at + n].double(), k, torch.nan_to_num(v), 0, -0.05, window)
+        # values of a lost block reach whoever sees one of its keys
+        t, j = torch.arange(lens[i])[:, None], torch.arange(lens[i])[None, :]
+        seen = (j <= t) & ((t - j < window) if window else True)
+        lost = torch.isnan(v).any(-1)  # [token, kv head]
+        hit = (seen.double() @ lost.double()).repeat_interleave(nh // 2, 1) > 0
+        want = torch.where(hit[..., None], torch.nan, want)
+        part = got[at + lead:at + n]
+        nan = torch.isnan(want)
+        assert torch.equal(nan, torch.isnan(part))
+        tol = tolerance(torch.nan_to_num(want), torch.nan_to_num(top), torch.nan_to_num(big), "bf16", lens[i], d)
+        assert ((part - want).abs() <= tol)[~nan].all()
+    f.cache.check()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_rows_that_see_nothing_and_lost_blocks(cuda_device, dtype):
     f = Filled([40, 300], 2, 128, dtype, "i8")
