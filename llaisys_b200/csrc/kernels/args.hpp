@@ -63,6 +63,7 @@ struct QuantView {
     const int32_t *block_table = nullptr; // [table_rows][table_stride]
     int32_t table_rows = 0, table_stride = 0;
     bool f8 = false; // codes are e4m3 numbers, not integers
+    bool overlap_launch = false; // as in KVView
 };
 
 // The arrays of a step from its requests' lengths (see llaisysPagedPlanDev).

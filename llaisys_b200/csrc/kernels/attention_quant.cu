@@ -31,8 +31,8 @@ namespace llaisys::kernels {
 namespace {
 
 constexpr int kRows = 16;
-constexpr int kMinPiece = 16; // units of the shortest piece
-constexpr int kTileUnits = 12; // what a row tile costs besides its blocks, in units of a block's time
+constexpr int kMinPiece = 12; // units of the shortest piece
+constexpr int kTileUnits = 24; // what a row tile costs besides its blocks, in units of a block's time
 constexpr int kSnap = 8;       // a piece's border that comes this near a row tile's first or last block moves there: no fragments of a few blocks
 constexpr uint32_t kWaitLimit = 1u << 20;
 constexpr int kErrTimeout = 8;
@@ -50,7 +50,7 @@ struct Shape {
     static constexpr int kMergeStride = kMergeDims + 8;                       // floats between rows in the merge buffer: lanes 4 g + t store at banks 8 g + 2 t
     static constexpr int kRowThreads = kThreads / kRows, kStep = 4 * kRowThreads; // threads that load and store a row, four dims each; dims between theirs
     static constexpr size_t kMerge = size_t(kWarps) * kSlots * kTile, kStats = kMerge + size_t(kWarps) * kRows * kMergeStride * 4;
-    static constexpr size_t kBars = kStats + 3 * kWarps * kRows * 4, kWords = kBars + kWarps * kSlots * 8, kPlaces = kWords + 32 + 3 * kRows * 4;
+    static constexpr size_t kBars = kStats + 3 * kWarps * kRows * 4, kWords = kBars + kWarps * kSlots * 8, kPlaces = kWords + 96 + 3 * kRows * 4;
     static constexpr size_t kPending = kPlaces + kWarps * kPlaceBytes; // fragments of tiles that other CTAs have parts of: at most two
     static constexpr size_t kRaw = kPending + 256;                     // the next tile's query rows as they are
     static constexpr size_t kQuery = kMerge; // 16 query rows as fragments, 32 bytes a dim, twice; the merge comes after their last use
@@ -70,6 +70,7 @@ struct QuantParams {
     const float *row_scale;
     int64_t out_stride;
     int32_t bf16; // of 16-bit activations: bfloat16
+    int32_t overlap;  // the launch may begin under the kernel in front of it
     int32_t out_wide; // four outputs of a row can be stored at once
     float *partials;
     int32_t *counters;
@@ -242,6 +243,13 @@ struct Place {
     Feed feed; // of the fragment ahead; now and next of the lanes beside it
     int now[32], next[32];
 };
+// The sequence of a piece's first unit, that sequence's first unit, and what is known of it.
+struct Start {
+    int64_t begin;
+    int a, seq;
+    SeqGeom g;
+};
+static_assert(sizeof(Start) <= 72, "shared memory");
 static_assert(sizeof(Place) <= kPlaceBytes && alignof(Place) == 8 && 2 * sizeof(Fragment) <= 256, "shared memory");
 template <typename S>
 __device__ __forceinline__ int tile_place(const QuantParams &p, const Feed &f, int k) { // -1: no page
@@ -264,9 +272,9 @@ __device__ __forceinline__ int tile_place(const QuantParams &p, const Feed &f, i
 }
 // first: the first of the fragment's blocks that is the warp's
 template <typename S>
-__device__ __forceinline__ Feed open_feed(const QuantParams &p, const Fragment &f, int first, int lane) {
+__device__ __forceinline__ Feed open_feed(const QuantParams &p, const Fragment &f, int seq, int first, int lane) {
     Feed feed;
-    const int seq = p.seq_ids[f.a], blocks = f.b1 - f.b0 - first, sweep = S::kPair * S::kWarps;
+    const int blocks = f.b1 - f.b0 - first, sweep = S::kPair * S::kWarps;
     feed.table = seq >= 0 && seq < p.kv.table_rows ? p.kv.block_table + int64_t(seq) * p.kv.table_stride : nullptr;
     feed.first = f.b0 + first;
     feed.count = blocks <= 0 ? 0 : blocks / sweep * S::kPair + min(blocks % sweep, S::kPair);
@@ -358,9 +366,9 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) attention
     extern __shared__ __align__(128) unsigned char smem[];
     float *s_merge = reinterpret_cast<float *>(smem + S::kMerge), *s_m = reinterpret_cast<float *>(smem + S::kStats);
     float *s_l = s_m + kWarps * kRows, *s_top = s_l + kWarps * kRows;
-    int64_t *s_start = reinterpret_cast<int64_t *>(smem + S::kWords); // sequence of the piece's first unit, that sequence's first unit
-    int *s_last = reinterpret_cast<int *>(s_start + 2);
-    float *s_factor = reinterpret_cast<float *>(s_start + 4), *s_lack = s_factor + kRows; // of the tile's rows
+    Start *s_start = reinterpret_cast<Start *>(smem + S::kWords);
+    int *s_last = reinterpret_cast<int *>(smem + S::kWords + 72); // [2]
+    float *s_factor = reinterpret_cast<float *>(smem + S::kWords + 96), *s_lack = s_factor + kRows; // of the tile's rows
     int *s_pos = reinterpret_cast<int *>(s_lack + kRows);
     uint32_t *s_query = reinterpret_cast<uint32_t *>(smem + S::kQuery); // [part][step][lane][4]
     const uint32_t query_u32 = smem_u32(s_query);
@@ -379,9 +387,15 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) attention
             }
             mbar_init_fence();
         }
+        // (launched programmatically: all but the set-up waits for the kernel in front; with overlap its index arrays are older than that kernel)
+        if (!p.overlap) {
+            grid_dependency_wait();
+        }
+        grid_launch_dependents();
         int64_t *sums = reinterpret_cast<int64_t *>(s_merge);
         const int per = (p.n_seqs + kThreads - 1) / kThreads, a0 = min(tid * per, p.n_seqs), a1 = min(a0 + per, p.n_seqs);
         int64_t mine = 0;
+        const int seq0 = a0 < a1 ? p.seq_ids[a0] : -1; // (on its way with the lengths)
         for (int a = a0; a < a1; ++a) {
             const SeqGeom g = seq_geom(p, a);
             mine += units_before(p, g, g.tiles) * p.kv.nkvh;
@@ -410,22 +424,20 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) attention
         }
         int64_t begin = before + upto - mine;
         if (begin <= w.pos && w.pos < begin + mine) {
-            int a = a0;
-            for (; a < a1; ++a) {
+            for (int a = a0; a < a1; ++a) {
                 const SeqGeom g = seq_geom(p, a);
                 const int64_t n = units_before(p, g, g.tiles) * p.kv.nkvh;
                 if (w.pos < begin + n) {
+                    *s_start = Start{begin, a, a == a0 ? seq0 : p.seq_ids[a], g};
                     break;
                 }
                 begin += n;
             }
-            s_start[0] = a;
-            s_start[1] = begin;
         }
         __syncthreads();
-        w.a = int(s_start[0]);
-        w.g = seq_geom(p, w.a);
-        const int64_t x = w.pos - s_start[1];
+        w.a = s_start->a;
+        w.g = s_start->g;
+        const int64_t x = w.pos - s_start->begin;
         int lo = 0, hi = w.g.tiles - 1; // last row tile whose first unit is not behind x
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
@@ -439,7 +451,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) attention
         w.blocks = tile_blocks(p, w.g, lo, w.gap);
         const int64_t in_front = units_before(p, w.g, lo) * p.kv.nkvh;
         w.kvh = int(x - in_front) / (w.blocks + kTileUnits);
-        w.first = s_start[1] + in_front + int64_t(w.kvh) * (w.blocks + kTileUnits);
+        w.first = s_start->begin + in_front + int64_t(w.kvh) * (w.blocks + kTileUnits);
     }
     Place &place = *reinterpret_cast<Place *>(smem + S::kPlaces + warp * kPlaceBytes);
     Feed feed;
@@ -468,7 +480,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) attention
                 }
             }
             cp_async_commit();
-            const Feed next = open_feed<S>(p, ahead, kPair * int((uint32_t(warp) - n) & (kWarps - 1u)), lane);
+            const Feed next = open_feed<S>(p, ahead, ahead.a == s_start->a ? s_start->seq : p.seq_ids[ahead.a], kPair * int((uint32_t(warp) - n) & (kWarps - 1u)), lane);
             place.now[lane] = next.now;
             place.next[lane] = next.next;
             if (lane == 0) {
@@ -513,6 +525,9 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) attention
         }
     };
     feed.count = 0;
+    if (p.overlap) {
+        grid_dependency_wait();
+    }
     more = step();
     __syncthreads(); // the sums' place is the queries'
     while (more) {
@@ -908,44 +923,66 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) attention
     }
 
     // ---- tiles that other CTAs have parts of: whoever comes last puts the parts together, in the order of the CTAs
+    const auto first_of = [&](const Fragment &f) { return int((f.first + snap_of(f.blocks)) / piece); };
+    const auto last_of = [&](const Fragment &f) { return int((f.first + f.blocks - snap_of(f.blocks) - 1) / piece); };
+    __syncthreads();
+    if (lane == 0 && warp < pending) { // (one release for everybody's parts: the barrier made them this thread's to publish)
+        const Fragment f = s_pending[warp];
+        int *counter = p.counters + first_of(f), seen;
+        asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;\n" : "=r"(seen) : "l"(counter) : "memory");
+        const bool last = seen == last_of(f) - first_of(f);
+        if (last) {
+            *counter = 0;
+        }
+        s_last[warp] = last;
+    }
     __syncthreads();
     for (int k = 0; k < pending; ++k) {
-        const Fragment f = s_pending[k];
-        const int c_first = int((f.first + snap_of(f.blocks)) / piece), c_last = int((f.first + f.blocks - snap_of(f.blocks) - 1) / piece);
-        if (tid == 0) {
-            __threadfence(); // (of everybody's parts: they were written before the barrier)
-            const int seen = atomicAdd(p.counters + c_first, 1);
-            *s_last = seen == c_last - c_first;
-            if (*s_last) {
-                p.counters[c_first] = 0;
-            }
-            __threadfence();
-        }
-        __syncthreads();
-        const bool last = *s_last != 0;
-        __syncthreads();
-        if (!last) {
+        if (!s_last[k]) {
             continue;
         }
+        const Fragment f = s_pending[k];
+        const int c_first = first_of(f), c_last = last_of(f);
         const int my_packed = f.row0 + my_row, my_query = my_packed / p.group, my_head = f.kvh * p.group + my_packed - my_query * p.group;
         const int64_t my_o = int64_t(f.q_start + my_query) * p.nh + my_head, my_out = int64_t(f.q_start + my_query) * p.out_stride + int64_t(my_head) * d;
+        // one pass, two parts' loads at a time
         float m_tile = -INFINITY, l_tile = 0.f, top_tile = -INFINITY;
-        for (int c = c_first; c <= c_last; ++c) {
-            const float *stats = p.partials + (int64_t(c) * 2 + (c == c_first ? 1 : 0)) * partial_floats(d) + kRows * d;
-            m_tile = fmaxf(m_tile, __ldcg(stats + my_row));
-            top_tile = fmaxf(top_tile, __ldcg(stats + 2 * kRows + my_row));
-        }
         float4 sum[D / S::kStep] = {};
-        for (int c = c_first; c <= c_last; ++c) {
-            const float *from = p.partials + (int64_t(c) * 2 + (c == c_first ? 1 : 0)) * partial_floats(d);
-            const float to = m_tile == -INFINITY ? 1.f : fast_exp2(__ldcg(from + kRows * d + my_row) - m_tile);
-            l_tile += __ldcg(from + kRows * d + kRows + my_row) * to;
+        for (int c = c_first; c <= c_last; c += 2) {
+            float m_part[2], l_part[2];
+            float4 x[2][D / S::kStep];
 #pragma unroll
-            for (int i = 0; i < D / S::kStep; ++i) {
-                const int dim = S::kStep * i + 4 * my_part;
-                if (dim < d) {
-                    const float4 x = __ldcg(reinterpret_cast<const float4 *>(from + my_row * d + dim));
-                    sum[i].x += x.x * to, sum[i].y += x.y * to, sum[i].z += x.z * to, sum[i].w += x.w * to;
+            for (int u = 0; u < 2; ++u) {
+                m_part[u] = -INFINITY;
+                l_part[u] = 0.f;
+                if (c + u <= c_last) {
+                    const float *from = p.partials + (int64_t(c + u) * 2 + (c + u == c_first ? 1 : 0)) * partial_floats(d), *stats = from + kRows * d;
+                    m_part[u] = __ldcg(stats + my_row);
+                    l_part[u] = __ldcg(stats + kRows + my_row);
+                    top_tile = fmaxf(top_tile, __ldcg(stats + 2 * kRows + my_row));
+#pragma unroll
+                    for (int i = 0; i < D / S::kStep; ++i) {
+                        const int dim = S::kStep * i + 4 * my_part;
+                        x[u][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (dim < d) {
+                            x[u][i] = __ldcg(reinterpret_cast<const float4 *>(from + my_row * d + dim));
+                        }
+                    }
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                if (c + u > c_last) {
+                    continue;
+                }
+                const float m_new = fmaxf(m_tile, m_part[u]);
+                const float had = m_tile == m_new ? 1.f : fast_exp2(m_tile - m_new), adds = m_part[u] == m_new ? 1.f : fast_exp2(m_part[u] - m_new);
+                m_tile = m_new;
+                l_tile = l_tile * had + l_part[u] * adds;
+#pragma unroll
+                for (int i = 0; i < D / S::kStep; ++i) {
+                    sum[i].x = sum[i].x * had + x[u][i].x * adds, sum[i].y = sum[i].y * had + x[u][i].y * adds;
+                    sum[i].z = sum[i].z * had + x[u][i].z * adds, sum[i].w = sum[i].w * had + x[u][i].w * adds;
                 }
             }
         }
@@ -993,6 +1030,7 @@ void attention_quant(stream_t stream, llaisysDataType_t dtype, const QuantView &
     p.out_stride = out.row_stride ? out.row_stride : int64_t(batch.nh) * kv.d;
     p.bf16 = dtype == LLAISYS_DTYPE_BF16;
     p.out_wide = reinterpret_cast<uintptr_t>(out.out) % (dtype == LLAISYS_DTYPE_F32 ? 16 : 8) == 0 && p.out_stride % 4 == 0;
+    p.overlap = kv.overlap_launch;
     p.partials = scratch.partials;
     p.counters = scratch.counters;
     p.error_flag = scratch.error_flag;
@@ -1006,7 +1044,7 @@ void attention_quant(stream_t stream, llaisysDataType_t dtype, const QuantView &
         auto start = [&](auto kernel) {
             const size_t bytes = Shape<D>::bytes(dtype == LLAISYS_DTYPE_F32);
             LLAISYS_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes)));
-            kernel<<<unsigned(counters), Shape<D>::kThreads, bytes, static_cast<cudaStream_t>(stream)>>>(p);
+            launch_programmatic_smem(kernel, dim3(unsigned(counters)), unsigned(Shape<D>::kThreads), bytes, static_cast<cudaStream_t>(stream), p);
         };
         auto pick = [&](auto exact) {
             constexpr bool kExact = decltype(exact)::value;

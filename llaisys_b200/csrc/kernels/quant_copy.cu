@@ -338,6 +338,8 @@ __global__ void __launch_bounds__(kWarps * 32, 8) quant_append_kernel(QuantView 
     if (row0 >= n_rows) {
         return;
     }
+    grid_dependency_wait(); // (launched programmatically: under the tail of the kernel in front)
+    grid_launch_dependents();
     const unsigned char *rows = reinterpret_cast<const unsigned char *>((is_v ? v_rows : k_rows) + int64_t(head) * kv.d);
     const int64_t row_step = int64_t(kv.nkvh) * row_bytes;
     // the rows are on their way before their place in the pool is looked up
@@ -478,8 +480,8 @@ void quant_append(stream_t stream, llaisysDataType_t dtype, const QuantView &kv,
         auto kernel = kv.f8 ? quant_append_kernel<T, true> : quant_append_kernel<T, false>;
         const int bytes = kWarps * append_smem(kv.d, sizeof(T));
         LLAISYS_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-        kernel<<<blocks, kWarps * 32, bytes, static_cast<cudaStream_t>(stream)>>>(kv, static_cast<const T *>(k_rows), static_cast<const T *>(v_rows), seq_ids,
-                                                                                  positions, n_rows, chunk, error_flag);
+        launch_programmatic_smem(kernel, dim3(blocks), kWarps * 32, size_t(bytes), static_cast<cudaStream_t>(stream), kv, static_cast<const T *>(k_rows),
+                                 static_cast<const T *>(v_rows), seq_ids, positions, n_rows, chunk, error_flag);
     });
     check_launch("quant_append");
 }

@@ -541,6 +541,7 @@ kernels::QuantView PagedKV::quantView(size_t layer) const {
     v.table_rows = int32_t(_cfg.max_seqs);
     v.table_stride = int32_t(_cfg.max_pages_per_seq);
     v.f8 = _cfg.store == LLAISYS_DTYPE_F8;
+    v.overlap_launch = _overlap;
     return v;
 }
 
