@@ -800,14 +800,15 @@ __global__ void __launch_bounds__(kThreads, 1) attention_quant_tc_kernel(QuantCh
                 l *= alpha;
                 if (i >= 1 && __any_sync(0xffffffffu, grow)) { // (the first product of a fragment overwrites O)
 #pragma unroll
-                    for (int c = 0; c < D / 32; ++c) {
-                        float v[32];
-                        tmem_ld32(tmem_o + c * 32, v);
+                    for (int c = 0; c < D / 16; ++c) { // (16 columns at a time: 32 beside the scores would spill)
+                        float v[16];
+                        tmem_ld16(tmem_o + c * 16, v);
+                        tmem_wait_ld();
 #pragma unroll
-                        for (int k = 0; k < 32; ++k) {
+                        for (int k = 0; k < 16; ++k) {
                             v[k] *= alpha;
                         }
-                        tmem_st32(tmem_o + c * 32, v);
+                        tmem_st16(tmem_o + c * 16, v);
                     }
                 }
                 const float neg_m = m_used == -INFINITY ? 0.f : kShift - m_used;
