@@ -432,11 +432,21 @@ __global__ void __launch_bounds__(kThreads, 1) attention_quant_tc_kernel(QuantCh
             constexpr int kHalfVecs = kVecs / 2; // 16-byte loads of a unit of V from either tile
             uint4 raw[2 * kHalfVecs];
             const uint4 none = kF8 ? make_uint4(0, 0, 0, 0) : make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
-            auto code_at = [&](int b, int at) { // 16 bytes of tile b
-                return tiles[b] >= 0 ? __ldcg(reinterpret_cast<const uint4 *>(p.kv.base + (long long)tiles[b] * tile_bytes) + at + lane) : none;
+            // Where the next unit's words come from: the low half of `raw` from one place on, the high half from another (null: no tile).
+            const uint4 *from[2] = {nullptr, nullptr};
+            auto tile_of = [&](int b) { return tiles[b] >= 0 ? reinterpret_cast<const uint4 *>(p.kv.base + (long long)tiles[b] * tile_bytes) + lane : nullptr; };
+            auto point_k = [&](int b) {
+                from[0] = tile_of(b);
+                from[1] = from[0] != nullptr ? from[0] + 32 * kHalfVecs : nullptr;
             };
-            auto fetch_k = [&](int b, int v) { raw[v] = code_at(b, 32 * v); };
-            auto fetch_v = [&](int half, int k) { raw[k] = code_at(k / kHalfVecs, kQuantTokens * D / 16 + 32 * (half * kHalfVecs + k % kHalfVecs)); };
+            auto point_v = [&](int half) {
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    from[b] = tile_of(b);
+                    from[b] = from[b] != nullptr ? from[b] + kQuantTokens * D / 16 + 32 * kHalfVecs * half : nullptr;
+                }
+            };
+            auto fetch = [&](int k) { raw[k] = from[k / kHalfVecs] != nullptr ? __ldcg(from[k / kHalfVecs] + 32 * (k % kHalfVecs)) : none; };
             int stage = 0;
             uint32_t turn = 0;
             auto take_stage = [&]() {
@@ -456,20 +466,21 @@ __global__ void __launch_bounds__(kThreads, 1) attention_quant_tc_kernel(QuantCh
                     ++turn;
                 }
             };
-            // K of block b of the two, word j of vector v
-            auto put_k = [&](uint32_t to, int b, int v, const uint4 &x) {
+            // K of a block, vector v
+            auto put_k = [&](uint32_t to, int v, const uint4 &x) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const uint32_t u = j == 0 ? (odd ? x.z : x.x) : j == 1 ? (odd ? x.w : x.y) : j == 2 ? (odd ? x.x : x.z) : (odd ? x.y : x.w);
                     // (bits 4 to 6 of a row's place are swizzled: 32 dims are bit 6, 16 dims bit 5, two tokens bit 5 and a row of 256 bytes on)
-                    sts64(to + (v >> 1) * kKPiece + b * 32 * 128 + (j & 1) * 256 + (k_at ^ uint32_t(((v & 1) << 6) | (((j >> 1) ^ (j & 1)) << 5))),
+                    sts64(to + (v >> 1) * kKPiece + (j & 1) * 256 + (k_at ^ uint32_t(((v & 1) << 6) | (((j >> 1) ^ (j & 1)) << 5))),
                           widen<kF8>(u));
                 }
             };
             step();
+            point_k(0);
 #pragma unroll
             for (int v = 0; v < kVecs; ++v) {
-                fetch_k(0, v);
+                fetch(v);
             }
             while (more && ok) {
                 // ---- K of the block
@@ -489,15 +500,18 @@ __global__ void __launch_bounds__(kThreads, 1) attention_quant_tc_kernel(QuantCh
                     mbar_arrive(bar(kBarRead + heard % kFeedSlots));
                 }
                 ++heard;
+#pragma unroll 1
+                for (int b = 0; b < 2; ++b) { // (the code of these warps shares the SM's instruction cache with the softmax: units in loops)
+                    if (b == 0) {
+                        point_k(1);
+                    } else {
+                        point_v(0);
+                    }
 #pragma unroll
-                for (int v = 0; v < kVecs; ++v) {
-                    put_k(to, 0, v, raw[v]);
-                    fetch_k(1, v);
-                }
-#pragma unroll
-                for (int v = 0; v < kVecs; ++v) {
-                    put_k(to, 1, v, raw[v]);
-                    fetch_v(0, v);
+                    for (int v = 0; v < kVecs; ++v) {
+                        put_k(to + b * 32 * 128, v, raw[v]);
+                        fetch(v);
+                    }
                 }
                 give_stage();
                 // ---- V of the block
@@ -505,10 +519,17 @@ __global__ void __launch_bounds__(kThreads, 1) attention_quant_tc_kernel(QuantCh
                 if (!ok) {
                     break;
                 }
-#pragma unroll
+#pragma unroll 1
                 for (int half = 0; half < 2; ++half) {
-                    if (half == 1) {
-                        step(); // (V is asked for; K of the next block comes next)
+                    if (half == 0) {
+                        point_v(1);
+                    } else {
+                        step(); // (V is asked for; K of the next block comes next, or nothing)
+                        if (more) {
+                            point_k(0);
+                        } else {
+                            from[0] = from[1] = nullptr;
+                        }
                     }
 #pragma unroll
                     for (int v = 0; v < kHalfVecs; ++v) {
@@ -516,17 +537,12 @@ __global__ void __launch_bounds__(kThreads, 1) attention_quant_tc_kernel(QuantCh
                         for (int j = 0; j < 4; ++j) {
                             const uint4 &a = raw[v], &c = raw[kHalfVecs + v];
                             const uint32_t x = j == 0 ? a.x : j == 1 ? a.y : j == 2 ? a.z : a.w, y = j == 0 ? c.x : j == 1 ? c.y : j == 2 ? c.z : c.w;
-                            const uint32_t row = to + (32 * (half * kHalfVecs + v) + 8 * j) * 128;
+                            const uint32_t row = to + half * (32 * kHalfVecs * 128) + (32 * v + 8 * j) * 128;
                             sts64(row + v_at, widen<kF8>(odd ? y : x));
                             sts64(row + (v_at ^ 64u), widen<kF8>(odd ? x : y));
                         }
-                        if (half == 0) {
-                            fetch_v(1, v);
-                            fetch_v(1, kHalfVecs + v);
-                        } else if (more) {
-                            fetch_k(0, v);
-                            fetch_k(0, kHalfVecs + v);
-                        }
+                        fetch(v);
+                        fetch(kHalfVecs + v);
                     }
                 }
                 give_stage();
@@ -799,7 +815,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_quant_tc_kernel(QuantCh
                 }
                 l *= alpha;
                 if (i >= 1 && __any_sync(0xffffffffu, grow)) { // (the first product of a fragment overwrites O)
-#pragma unroll
+#pragma unroll 1
                     for (int c = 0; c < D / 16; ++c) { // (16 columns at a time: 32 beside the scores would spill)
                         float v[16];
                         tmem_ld16(tmem_o + c * 16, v);
