@@ -225,7 +225,7 @@ LLAISYS_API int llaisysPagedKVAppendDev(llaisysPagedKV_t kv, size_t layer, const
                                         const int32_t *seq_ids_dev, const int32_t *positions_dev, size_t n_rows,
                                         llaisysStream_t stream);
 /* Inverse of llaisysPagedKVAppendDev: token positions_dev[i] of sequence seq_ids_dev[i] -> row i of k_out, v_out [n_rows, nkvh, head_dim],
- * in any order. Rows whose sequence or position does not exist are left as they were. */
+ * in any order. Rows whose sequence or position does not exist are left as they were and reported by llaisysPagedKVCheck. */
 LLAISYS_API int llaisysPagedKVGatherDev(llaisysPagedKV_t kv, size_t layer, void *k_out, void *v_out, const int32_t *seq_ids_dev,
                                         const int32_t *positions_dev, size_t n_rows, llaisysStream_t stream);
 /* The step before attention, fused: qkv is the packed q|k|v projection [n_rows, (nh + 2 nkvh) * head_dim] of the cache's
@@ -270,7 +270,7 @@ LLAISYS_API int llaisysPagedAttentionPrefillDev(llaisysPagedKV_t kv, size_t laye
  *   block_table_dev [table_rows][table_stride]: entries [pages(held), pages(held + new)) of request i, requests in order, take
  *                                 free_pages_dev[0], [1], ...; NULL free_pages_dev: the table is complete already and only read
  *   status_dev [2]                pages taken, and LLAISYS_PLAN_ bits
- * Any output may be NULL, and so may the table when neither slots nor growth are wanted. Rows behind the last request's, up to n_rows, are -1
+ * Any output may be NULL, and so may the table when neither slots nor growth are wanted; no output lies over an input. Rows behind the last request's, up to n_rows, are -1
  * (such rows are skipped by appends to a cache held in 8 bits). A request may appear once.
  * What cannot be done is left out and flagged, never written elsewhere: too few free pages take none at all (slots on missing pages are -1);
  * rows behind n_rows are dropped (q_starts ends at n_rows); negative counts and sums over 2^31 - 1 count as nothing brought; a request whose row

@@ -11,6 +11,7 @@
 #include "../kernels/kernels.hpp"
 #endif
 
+#include <algorithm>
 #include <string>
 
 namespace {
@@ -133,6 +134,28 @@ int llaisysPagedPlanDev(llaisysDeviceType_t device_type, int device_id, const Ll
         }
         if (a->block_table_dev == nullptr && (a->row_slots_dev != nullptr || a->free_pages_dev != nullptr)) {
             throw StatusError(LLAISYS_E_INVALID, "paged plan: slots and growth need the block table");
+        }
+        // arrays that a CTA may still read while another one writes: all outputs lie apart from the inputs
+        struct Array {
+            const void *at;
+            size_t count, elem;
+        };
+        const Array in[] = {{a->seq_ids_dev, a->n_seqs, 4}, {a->held_dev, a->n_seqs, 4}, {a->new_dev, a->n_seqs, 4}, {a->free_pages_dev, a->n_free, 4},
+                            {a->block_table_dev, std::min(a->table_rows * a->table_stride, size_t(1) << 60), 4}};
+        const Array out[] = {{a->q_starts_dev, a->n_seqs + 1, 4}, {a->kv_lens_dev, a->n_seqs, 4}, {a->page_starts_dev, a->n_seqs + 1, 4},
+                             {a->row_seqs_dev, a->n_rows, 4}, {a->row_positions_dev, a->n_rows, 4}, {a->row_slots_dev, a->n_rows, 8}, {a->status_dev, 2, 4}};
+        const auto apart = [](const Array &x, const Array &y) {
+            const uintptr_t from = reinterpret_cast<uintptr_t>(x.at), other = reinterpret_cast<uintptr_t>(y.at);
+            return x.at == nullptr || y.at == nullptr || from + x.count * x.elem <= other || other + y.count * y.elem <= from;
+        };
+        for (const Array &x : in) {
+            bool ok = reinterpret_cast<uintptr_t>(x.at) % x.elem == 0 && (&x == &in[4] || a->free_pages_dev == nullptr || apart(x, in[4]));
+            for (const Array &y : out) {
+                ok = ok && reinterpret_cast<uintptr_t>(y.at) % y.elem == 0 && apart(x, y);
+            }
+            if (!ok) {
+                throw StatusError(LLAISYS_E_INVALID, "paged plan: an array is not aligned to its elements, or an output lies over an input");
+            }
         }
         if (device_type != LLAISYS_DEVICE_NVIDIA) {
             throw StatusError(LLAISYS_E_UNSUPPORTED, "paged plan: NVIDIA devices only");

@@ -185,7 +185,8 @@ __device__ __forceinline__ bool next_fragment(const QuantParams &p, Walker &w, F
         f.rows = min(kRows, w.g.q_len * p.group - f.row0);
         f.kvh = w.kvh;
         f.b0 = at;
-        f.b1 = min(to, w.blocks);
+        // (a last tile of fewer than 16 rows is counted as a full one, whose rows would see keys behind the sequence)
+        f.b1 = max(min(min(to, w.blocks), (w.g.tokens + kQuantTokens - 1) / kQuantTokens - w.gap), at);
         f.gap = w.gap;
         f.kept = w.gap > 0 ? (p.keep_first + kQuantTokens - 1) / kQuantTokens : 0;
         f.begins = at == 0;
@@ -427,8 +428,11 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) attention
         piece = max((line + gridDim.x - 1) / gridDim.x, int64_t(kMinPiece));
         w.pos = min(piece * blockIdx.x, line);
         w.end = min(w.pos + piece, line);
-        if (w.pos >= w.end) {
-            return; // (the whole CTA)
+        if (w.pos >= w.end) { // (the whole CTA)
+            if (p.overlap) { // where nobody has work the launch still ends behind the kernel in front
+                grid_dependency_wait();
+            }
+            return;
         }
         int64_t begin = before + upto - mine;
         if (begin <= w.pos && w.pos < begin + mine) {
@@ -458,7 +462,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) attention
         w.tile = lo;
         w.blocks = tile_blocks(p, w.g, lo, w.gap);
         const int64_t in_front = units_before(p, w.g, lo) * p.kv.nkvh;
-        w.kvh = int(x - in_front) / (w.blocks + kTileUnits);
+        w.kvh = int((x - in_front) / (w.blocks + kTileUnits));
         w.first = s_start->begin + in_front + int64_t(w.kvh) * (w.blocks + kTileUnits);
     }
     Place &place = *reinterpret_cast<Place *>(smem + S::kPlaces + warp * kPlaceBytes);
@@ -1084,7 +1088,9 @@ void attention_quant(stream_t stream, llaisysDataType_t dtype, const QuantView &
     p.counters = scratch.counters;
     p.error_flag = scratch.error_flag;
     CHECK_ARGUMENT(aligned16(q), "attention: queries must be 16-byte aligned");
-    CHECK_ARGUMENT(int64_t(batch.total_q) * p.group <= 0x7fffffff - kRows, "attention: too many rows for one launch");
+    CHECK_ARGUMENT(int64_t(batch.total_q) * p.group <= 0x7fffffff - kRows && batch.n_seqs <= 1 << 30 &&
+                       int64_t(kv.table_stride) * kv.blocks_per_page * p.group <= 1 << 30,
+                   "attention: too many rows or tokens for one launch");
     size_t floats, counters;
     attention_quant_scratch(kv.d, &floats, &counters);
     CHECK_ARGUMENT(scratch.partials_floats >= floats && scratch.counters_len >= counters, "attention: workspace too small");

@@ -66,7 +66,7 @@ struct QuantChunkParams {
     const int32_t *seq_ids, *kv_lens, *q_starts;
     int32_t table_stride; // of the block table, in blocks of 16 tokens
     int32_t contiguous, const_q_len, const_kv_len; // (of the other kernel's line: always a pool here)
-    int32_t n_seqs, nkvh, group, nh;
+    int32_t n_seqs, total_q, nkvh, group, nh;
     uint32_t group_inverse; // ceil(2^32 / group)
     const void *q;
     void *out;
@@ -1028,9 +1028,12 @@ bool attention_quant_tc(stream_t stream, llaisysDataType_t dtype, const QuantVie
                         const AttnOut &out, const AttnScratch &scratch) {
     const bool bf16 = dtype == LLAISYS_DTYPE_BF16;
     const int group = batch.nh / kv.nkvh;
+    // the line's units, whatever lengths the arrays hold, and its geometry are counted in 32 bits
+    const int64_t longest = std::max(int64_t(kv.table_stride) * kv.blocks_per_page * kPage, int64_t(batch.total_q));
+    const int64_t most_tiles = int64_t(batch.total_q) * group / kRows + batch.n_seqs;
     if (!(bf16 || dtype == LLAISYS_DTYPE_F16) || (kv.d != 64 && kv.d != 128) || batch.q_starts == nullptr || out.out == nullptr || out.part != nullptr ||
         group > 32 || int64_t(batch.total_q) * group >= int64_t(1) << 26 || !aligned16(q) || !aligned16(out.out) || out.row_stride % 8 != 0 ||
-        int64_t(kv.table_stride) * kv.blocks_per_page * kPage > 0x7fffffff || !wide_tiles_pay(batch, kv.nkvh, group)) {
+        longest * group >= int64_t(1) << 30 || most_tiles > (int64_t(1) << 30) / ((longest / kKeys + 1 + kTileCost) * kv.nkvh) || !wide_tiles_pay(batch, kv.nkvh, group)) {
         return false;
     }
     size_t floats, counters;
@@ -1045,6 +1048,7 @@ bool attention_quant_tc(stream_t stream, llaisysDataType_t dtype, const QuantVie
     p.q_starts = batch.q_starts;
     p.table_stride = kv.table_stride * kv.blocks_per_page;
     p.n_seqs = batch.n_seqs;
+    p.total_q = batch.total_q;
     p.nkvh = kv.nkvh;
     p.group = group;
     p.nh = batch.nh;

@@ -2,7 +2,7 @@
 //
 // Rows are packed over queries and the heads of a group, 256 of a sequence and kv head are a tile, and a tile visits its visible keys 128 at a
 // time. P, the parameters of a kernel, names: kv_lens, q_starts, n_seqs, nkvh, group, window, keep_first, table_stride (pages of 16 tokens),
-// contiguous, const_q_len, const_kv_len; kQueriesMayLead: chunks may be longer than what their sequence holds.
+// contiguous, const_q_len, const_kv_len; kQueriesMayLead: chunks may be longer than what their sequence holds, and end with total_q.
 #pragma once
 
 #include "device_utils.cuh"
@@ -34,7 +34,13 @@ __device__ __forceinline__ SeqGeom seq_geom(const P &p, int a) {
     } else {
         g.q_start = p.q_starts[a];
         g.q_len = p.q_starts[a + 1] - g.q_start;
-        g.kv_len = P::kQueriesMayLead ? max(min(p.kv_lens[a], p.table_stride * kPage), g.q_len) : min(max(p.kv_lens[a], g.q_len), p.table_stride * kPage);
+        if constexpr (P::kQueriesMayLead) {
+            g.q_start = max(g.q_start, 0);
+            g.q_len = max(min(p.q_starts[a + 1], p.total_q) - g.q_start, 0);
+            g.kv_len = max(min(p.kv_lens[a], p.table_stride * kPage), g.q_len);
+        } else {
+            g.kv_len = min(max(p.kv_lens[a], g.q_len), p.table_stride * kPage);
+        }
     }
     g.q_len = min(g.q_len, g.kv_len); // (a chunk longer than the tables can hold: flagged elsewhere, never off the end here)
     g.off = g.kv_len - g.q_len;

@@ -83,7 +83,8 @@ __global__ void __launch_bounds__(kThreads) paged_plan_kernel(PlanArgs p) {
     if (tid == 0) {
         s_flags = 0;
     }
-    const int per = (p.n_seqs + kThreads - 1) / kThreads, i0 = min(tid * per, p.n_seqs), i1 = min(i0 + per, p.n_seqs);
+    const int per = int((int64_t(p.n_seqs) + kThreads - 1) / kThreads), i0 = int(min(int64_t(tid) * per, int64_t(p.n_seqs)));
+    const int i1 = i0 + min(per, p.n_seqs - i0);
     int flags = 0;
     int64_t mine[3] = {0, 0, 0}; // rows, pages, pages taken
     for (int i = i0; i < i1; ++i) {

@@ -88,6 +88,7 @@ PagedKV::PagedKV(const PagedKVConfig &cfg) : _cfg(cfg) {
         l.page_elems = l.nkvh * cfg.page_size * (l.k_row + l.v_row);
         l.offset = pool_bytes;
         l.page_bytes = quantized() ? cfg.page_size / kQuantBlock * l.nkvh * quantTileBytes(l.k_dim) : l.page_elems * _elem;
+        KV_REQUIRE(!quantized() || l.page_bytes <= (size_t(1) << 48) / cfg.num_pages / cfg.nlayer, LLAISYS_E_INVALID, "paged KV: pool too large");
         l.bytes = cfg.num_pages * l.page_bytes;
         pool_bytes += (l.bytes + 255) / 256 * 256;
         max_kvh = std::max(max_kvh, l.nkvh);
@@ -787,6 +788,7 @@ void PagedKV::normAppendDev(size_t layer, const kernels::NormAppendArgs &args, l
 
 void PagedKV::latentAppendDev(size_t layer, const kernels::LatentAppendArgs &args, llaisysStream_t stream) {
     checkLayer(layer);
+    requireWide("latent append");
     const Layer &l = _layers[layer];
     KV_REQUIRE(args.n_rows <= kMaxInt32 && l.v_row == 0 && l.nkvh == 1 && args.rank > 0 && args.rot_dims >= 0 && args.rot_dims % 2 == 0 &&
                    size_t(args.rank) == l.v_dim && size_t(args.rank + args.rot_dims) == l.k_dim,
@@ -827,6 +829,7 @@ bool PagedKV::canExpand(size_t layer, size_t dim, size_t rot_dim, size_t vdim) c
 void PagedKV::latentGatherDev(size_t layer, void *out, int64_t out_stride, const int32_t *seq_ids_dev, const int32_t *page_starts_dev,
                               const int32_t *kv_lens_dev, size_t n_seqs, size_t max_kv_len, llaisysStream_t stream) {
     checkLayer(layer);
+    requireWide("latent gather");
     KV_REQUIRE(onDevice() && _layers[layer].v_row == 0 && out_stride >= int64_t(_layers[layer].k_dim), LLAISYS_E_INVALID,
                "paged KV latent gather: this layer holds no latents of this size");
     KV_REQUIRE(max_kv_len <= _cfg.page_size * _cfg.max_pages_per_seq, LLAISYS_E_INVALID, "paged KV latent gather: context too large for this cache");
@@ -840,6 +843,7 @@ void PagedKV::latentGatherDev(size_t layer, void *out, int64_t out_stride, const
 }
 
 void PagedKV::expandedDev(const kernels::ExpandedArgs &args, llaisysStream_t stream) {
+    requireWide("expanded attention");
 #ifdef ENABLE_NVIDIA_API
     KV_REQUIRE(onDevice(), LLAISYS_E_UNSUPPORTED, "expanded attention: NVIDIA caches only");
     enter();
@@ -909,6 +913,7 @@ void PagedKV::decodeSplitDev(size_t layer, const void *q, const int32_t *seq_ids
                              size_t n_seqs, size_t max_kv_len, size_t nh, float scale, const kernels::PeerSink &peers,
                              llaisysStream_t stream) {
     checkLayer(layer);
+    requireWide("split decode");
     KV_REQUIRE(nh > 0 && nh % _layers[layer].nkvh == 0, LLAISYS_E_INVALID, "split decode: nh = ", nh, " is not a multiple of nkvh = ",
                _layers[layer].nkvh);
     KV_REQUIRE(n_seqs >= 1 && n_seqs <= kMaxDecodeSeqs && max_kv_len <= _cfg.page_size * _cfg.max_pages_per_seq,

@@ -401,6 +401,20 @@ def test_rows_that_see_nothing_and_lost_blocks(cuda_device, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,nh,nkvh,d", [("bf16", 2, 2, 128), ("f16", 4, 1, 64), ("f32", 12, 2, 96), ("bf16", 16, 1, 256)])
+def test_tables_that_are_full(cuda_device, dtype, nh, nkvh, d):
+    """Sequences that end in the last block of their tables: nothing behind it is looked up."""
+    f = Filled([160, 159, 158, 157, 156, 145, 144], nkvh, d, dtype, "i8")
+    parts = [(i, 1) for i in range(7)]
+    f.check_attention(parts, nh)
+    f.check_attention(parts, nh, window=40, keep=20)
+    for n in (1, 2, 3, 5, 140):
+        f.check_attention([(i, n) for i, _ in parts], nh, chunks=True)
+        f.check_attention([(i, n) for i, _ in parts], nh, window=20, keep=3, chunks=True)
+    f.cache.check()
+
+
+@pytest.mark.gpu
 def test_one_long_sequence(cuda_device):
     f = Filled([70001], 1, 64, "bf16", "i8")
     f.check_attention([(0, 1)], 8)
@@ -557,6 +571,93 @@ def test_steps_planned_on_the_gpu_and_replayed(cuda_device, dtype, store):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,nh,d", [("bf16", 8, 128), ("f32", 4, 64)])
+def test_steps_with_launch_overlap(cuda_device, dtype, nh, d):
+    """Append and decode of every step launched under the kernels in front of them: the same bits, also behind calls in which nobody has a query."""
+    n, steps = 37, 6
+    rng = np.random.default_rng(2)
+    lens = rng.integers(1, 300, n).tolist()
+    most = max(lens) + steps
+    outs = []
+    for overlap in (False, True):
+        f = Filled(lens, 2, d, dtype, "i8", extra=steps)
+        f.cache.flush()
+        torch.manual_seed(9)
+        data = [tuple(torch.randn(n, h, d).to(TORCH[dtype]).cuda() for h in (2, 2, nh)) for _ in range(steps)]
+        ids = i32(f.seqs)
+        kv, pos = [i32([x + s + 1 for x in lens]) for s in range(steps)], [i32([x + s for x in lens]) for s in range(steps)]
+        out = torch.zeros(steps, n, nh, d, dtype=TORCH[dtype], device="cuda")
+        none = i32([0] * (n + 1))
+        torch.cuda.synchronize()
+        f.cache.set_launch_overlap(overlap)
+        for s, (k, v, q) in enumerate(data):
+            f.cache.append_dev(0, k, v, ids, pos[s], n, stream())
+            f.cache.attention_dev(0, out[s], q, ids, none, kv[s], n_seqs=n, total_q=n, max_q_len=1, max_kv_len=most, nh=nh, scale=0.1, stream=stream())
+            f.cache.decode_dev(0, out[s], q, ids, kv[s], n, most, nh, 0.1, stream())
+        f.cache.check()
+        outs.append(out.cpu())
+    assert torch.equal(*outs) and outs[0].abs().max() > 0
+
+
+@pytest.mark.gpu
+def test_two_caches_on_two_streams_and_graphs(cuda_device):
+    """Calls of two caches side by side, eager and replayed, give what they give alone."""
+    sides = []
+    for seed in (0, 1):
+        f = Filled([700, 20, 333], 2, 128, "bf16", "i8", extra=4, seed=seed)
+        f.cache.flush()
+        q = torch.randn(600, 16, 128, generator=torch.Generator().manual_seed(seed)).bfloat16().cuda()
+        sides.append((f, q, i32(f.seqs), i32([0, 400, 401, 600]), i32([700, 20, 333]), torch.cuda.Stream()))
+
+    def call(side, chunk, dec):
+        f, q, ids, starts, kv, _ = side
+        f.cache.attention_dev(0, chunk, q, ids, starts, kv, n_seqs=3, total_q=600, max_q_len=400, max_kv_len=700, nh=16, scale=0.1, stream=stream())
+        f.cache.decode_dev(0, dec, q, ids, kv, 3, 700, 16, 0.1, stream())
+
+    def outputs():
+        return [(torch.zeros_like(q), torch.zeros(3, 16, 128, dtype=q.dtype, device="cuda")) for _, q, *_ in sides]
+
+    alone, eager, replayed = outputs(), outputs(), outputs()
+    graphs = []
+    for side, a in zip(sides, alone):
+        call(side, *a)
+    torch.cuda.synchronize()
+    for side, r in zip(sides, replayed):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            call(side, *r)
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for side, e in zip(sides, eager):
+            with torch.cuda.stream(side[5]):
+                call(side, *e)
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for side, g in zip(sides, graphs):
+            with torch.cuda.stream(side[5]):
+                g.replay()
+    torch.cuda.synchronize()
+    for a, e, r in zip(alone, eager, replayed):
+        for x, y, z in zip(a, e, r):
+            assert torch.equal(x, y) and torch.equal(x, z)
+    for f, *_ in sides:
+        f.cache.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("held,rows", [(2000, 900), (40, 40)])
+def test_queries_end_with_the_call(cuda_device, held, rows):
+    """q_starts that go on behind total_q: the queries there are none of the call's."""
+    f = Filled([held], 2, 128, "bf16", "i8")
+    q = torch.randn(rows, 8, 128).bfloat16().cuda()
+    out, want = torch.full_like(q, 9.0), torch.empty(rows - 30, 8, 128, dtype=q.dtype, device="cuda")
+    kw = dict(n_seqs=1, max_q_len=rows, nh=8, scale=0.1, stream=stream())
+    f.cache.attention_dev(0, out, q, i32(f.seqs), i32([0, rows]), i32([held]), total_q=rows - 30, max_kv_len=held, **kw)
+    f.cache.attention_dev(0, want, q, i32(f.seqs), i32([0, rows - 30]), i32([held]), total_q=rows - 30, max_kv_len=held, **kw)
+    assert (out[rows - 30:] == 9).all() and torch.equal(out[:rows - 30], want)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 def test_gather_rows_of_a_plain_cache(cuda_device, dtype):
     cache = llaisys.PagedKVCache(9, 2, 64, dtype=NAMES[dtype], device=llaisys.DeviceType.NVIDIA, max_seqs=2)
@@ -609,10 +710,31 @@ def test_refusals_of_the_cache(changes, status):
                                             (dict(free_pages_dev=64), Status.INVALID), (dict(table_stride=1 << 33), Status.INVALID)])
 def test_refusals_of_the_plan(changes, status):
     args = LlaisysPagedPlan(**(dict(held_dev=64, new_dev=64, n_seqs=1, page_size=16, n_rows=1) | changes))
-    assert LIB_LLAISYS.llaisysPagedPlanDev(int(llaisys.DeviceType.NVIDIA), 0, ctypes.byref(args), None) == status
-    assert LIB_LLAISYS.llaisysPagedPlanDev(int(llaisys.DeviceType.NVIDIA), 0, None, None) == Status.INVALID
+    assert LIB_LLAISYS.llaisysPagedPlanDev(int(llaisys.DeviceType.CPU), 0, ctypes.byref(args), None) == status
+    assert LIB_LLAISYS.llaisysPagedPlanDev(int(llaisys.DeviceType.CPU), 0, None, None) == Status.INVALID
     args = LlaisysPagedPlan(held_dev=64, new_dev=64, n_seqs=1, page_size=16, n_rows=1)
     assert LIB_LLAISYS.llaisysPagedPlanDev(int(llaisys.DeviceType.CPU), 0, ctypes.byref(args), None) == Status.UNSUPPORTED
+
+
+@pytest.mark.parametrize("changes", [dict(kv_lens_dev=4096), dict(q_starts_dev=4100), dict(row_positions_dev=4076), dict(status_dev=8188), dict(held_dev=4098),
+                                     dict(row_slots_dev=65540, block_table_dev=1 << 20, table_rows=4, table_stride=4),
+                                     dict(row_seqs_dev=(1 << 20) + 60, block_table_dev=1 << 20, table_rows=4, table_stride=4),
+                                     dict(free_pages_dev=(1 << 20) + 60, n_free=1, block_table_dev=1 << 20, table_rows=4, table_stride=4)])
+def test_refusals_of_a_plan_whose_arrays_overlap_or_are_not_aligned(changes):
+    # (asked of a CPU, which has no such call: an argument that is not refused is never launched)
+    args = LlaisysPagedPlan(**(dict(held_dev=4096, new_dev=8192, n_seqs=2, page_size=16, n_rows=7) | changes))
+    assert LIB_LLAISYS.llaisysPagedPlanDev(int(llaisys.DeviceType.CPU), 0, ctypes.byref(args), None) == Status.INVALID
+
+
+def test_arrays_of_a_plan_may_lie_side_by_side():
+    args = LlaisysPagedPlan(held_dev=4096, new_dev=4104, n_seqs=2, page_size=16, n_rows=7, kv_lens_dev=4112, q_starts_dev=4084, status_dev=4120)
+    assert LIB_LLAISYS.llaisysPagedPlanDev(int(llaisys.DeviceType.CPU), 0, ctypes.byref(args), None) == Status.UNSUPPORTED
+
+
+def test_refusal_of_a_pool_beyond_64_bits():
+    with pytest.raises(llaisys.LlaisysError) as e:
+        llaisys.PagedKVCache.quantized(num_pages=2 ** 31 - 1, nkvh=65535, head_dim=256, page_size=2 ** 30, max_pages_per_seq=1)
+    assert e.value.status == Status.INVALID
 
 
 @pytest.mark.gpu
@@ -627,6 +749,10 @@ def test_refusals_of_calls_that_need_wide_pages(cuda_device):
              lambda c: c.decode_step_host(0, x.cpu(), x.cpu(), x.cpu(), x.cpu(), [0], [1], 4, 1.0),
              lambda c: c.fade_dev(0, x, x, zero, None, one, n_seqs=1, total_q=1, max_q_len=1, max_kv_len=1, nh=4, scale=1.0, stream=stream(), fade_a=x,
                                   fade_b=x),
+             lambda c: c.latent_append_dev(0, stream(), proj=x, q_norm=x, kv_norm=x, q_latent=x, seq_ids_dev=zero, positions_dev=zero, rank=128, nh=4,
+                                           n_rows=1),
+             lambda c: c.latent_gather_dev(0, x, 128, zero, zero, one, 1, 1, stream()),
+             lambda c: c.expanded_dev(stream(), q=x, k=x, k_shared=x, v=x, out=x, page_starts_dev=zero, q_starts_dev=zero, kv_lens_dev=one, nh=4, n_seqs=1),
              lambda c: c.gates_dev(0, x, x, zero, None, one, n_seqs=1, total_q=1, max_q_len=1, max_kv_len=1, nh=4, scale=1.0, stream=stream())]
     for call in calls:
         with pytest.raises(llaisys.LlaisysError) as e:
