@@ -19,6 +19,8 @@
 // A warp feeds itself: it has a ring of slots of its own, asks for a block as soon as it has read the one that lay in the slot, and looks one
 // fragment ahead, so that nothing but the merge makes warps meet; codes come out of a slot by 16-byte loads in the order the products want
 // them (quant_tile.cuh). (A ninth warp for the copies would leave 168 registers a thread instead of 255, and the accumulators spill.)
+// Measured: 64 sequences of 4096 tokens, 12 / 2 heads of 128, integers, 33 us (135 MB: 4.1 TB/s; the loop over blocks runs at about 6, the rest is the
+// start, the queries, the merge of the warps and the join of the 2.3 parts that a tile is in); one sequence of 777 tokens 10.3 us.
 // Waits for copies are bounded; one that runs out sets bit 8 of the error word, and the warp asks for nothing more.
 #include "kernels.hpp"
 #include "launch_utils.cuh"
@@ -43,12 +45,14 @@ constexpr float kShift = 14.f; // weights are 2^14 times what they stand for
 constexpr size_t kPlaceBytes = 512;
 
 // Heads of up to 128: two CTAs of four warps on an SM, each warp with two blocks at a time and 255 registers. Longer ones: one CTA of eight warps.
+// Three CTAs where 168 registers do (tiles of 8 rows, heads of up to 64): 24 sequences, windows of 2000 tokens, 24.7 us instead of 26.4; with heads of
+// 128 the shorter rings cost more than the third CTA brings, 64 sequences of 4096 tokens 33.8 us instead of 33.0.
 // R: rows that a warp multiplies at a time, 16 or 8 (see the kernel).
 template <int D, int R>
 struct Shape {
-    static constexpr int kCtas = D <= 128 ? 2 : 1, kWarps = D <= 128 ? 4 : 8, kThreads = kWarps * 32, kPair = D <= 128 ? 2 : 1;
+    static constexpr int kCtas = D <= 64 && R == 8 ? 3 : D <= 128 ? 2 : 1, kWarps = D <= 128 ? 4 : 8, kThreads = kWarps * 32, kPair = D <= 128 ? 2 : 1;
     static constexpr int kTile = 2 * kQuantTokens * D + 16;
-    static constexpr int kSlots = D <= 64 ? 8 : D <= 128 ? 4 : 2;             // of a warp
+    static constexpr int kSlots = D <= 64 ? kCtas == 3 ? 6 : 8 : D <= 128 ? 4 : 2;           // of a warp
     static constexpr int kMergeDims = D < 128 ? D : 128;                      // merged at a time
     // floats between rows in the merge buffer: lanes 4 g + t store at banks 8 g + 2 t (8 rows: 8 t + g)
     static constexpr int kMergeStride = kMergeDims + (R == 16 ? 8 : 4);
@@ -59,7 +63,7 @@ struct Shape {
     static constexpr size_t kRaw = kPending + 256;                     // the next tile's query rows as they are
     static constexpr size_t kQuery = kMerge; // query rows as fragments, 2 R bytes a dim, twice; the merge comes after their last use
     static constexpr size_t bytes(bool wide) { return kRaw + R * D * (wide ? 4 : 2); }
-    static_assert(2 * 2 * R * D <= kWarps * R * kMergeStride * 4 && kStats % 16 == 0 && bytes(true) <= (kCtas == 2 ? 113 : 227) * 1024 && kRaw % 16 == 0, "");
+    static_assert(2 * 2 * R * D <= kWarps * R * kMergeStride * 4 && kStats % 16 == 0 && bytes(true) <= 227 / kCtas * 1024 && kRaw % 16 == 0, "");
 };
 
 struct QuantParams {
@@ -1149,7 +1153,7 @@ __global__ void __launch_bounds__(Shape<D, R>::kThreads, Shape<D, R>::kCtas) att
 } // namespace
 
 void attention_quant_scratch(int32_t d, size_t *floats, size_t *counters) {
-    const size_t ctas = size_t(device_sms()) * (d <= 128 ? Shape<128, 16>::kCtas : Shape<256, 16>::kCtas);
+    const size_t ctas = size_t(device_sms()) * (d <= 64 ? Shape<64, 8>::kCtas : d <= 128 ? Shape<128, 8>::kCtas : Shape<256, 8>::kCtas);
     *floats = ctas * 2 * partial_floats(d);
     *counters = ctas;
 }
@@ -1191,7 +1195,7 @@ void attention_quant(stream_t stream, llaisysDataType_t dtype, const QuantView &
         auto start = [&](auto kernel) {
             const size_t bytes = Shape<D, R>::bytes(dtype == LLAISYS_DTYPE_F32);
             LLAISYS_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes)));
-            launch_programmatic_smem(kernel, dim3(unsigned(counters)), unsigned(Shape<D, R>::kThreads), bytes, static_cast<cudaStream_t>(stream), p);
+            launch_programmatic_smem(kernel, dim3(unsigned(device_sms() * Shape<D, R>::kCtas)), unsigned(Shape<D, R>::kThreads), bytes, static_cast<cudaStream_t>(stream), p);
         };
         auto pick = [&](auto exact) {
             constexpr bool kExact = decltype(exact)::value;

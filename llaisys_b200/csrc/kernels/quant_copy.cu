@@ -5,9 +5,12 @@
 // One warp per run, head and K or V: nobody else touches those codes or that scale, so there is nothing to order.
 //
 // Bound: bytes, rows in and codes out (and back the other way); for a token per sequence the chain of loads row -> table -> tile. A warp copies a
-// run to shared memory between the maximum and the rounding (asynchronously, while its place is looked up), so that rows are read once, and stores codes 16 bytes a lane in the order of the tile
-// (quant_tile.cuh): a lane of K takes the four neighbours that make a word of its own; one of V takes four tokens of four dims, turns its 4 x 4 codes
-// round and passes them on through shared memory.
+// run to shared memory between the maximum and the rounding (asynchronously, while its place is looked up), so that rows are read once, and stores
+// codes 16 bytes a lane in the order of the tile (quant_tile.cuh): a lane of K takes the four neighbours that make a word of its own; one of V takes
+// four tokens of four dims, turns its 4 x 4 codes round and passes them on through shared memory.
+// Measured: 65536 rows of 2 heads of 128 in bf16, integers, in and back out 42 us (101 MB each way: 4.8 TB/s, bound by issue: a number costs its
+// maximum, a product, a rounding and its share of the byte moves); 64 rows of 64 sequences 7.5 us for both. (Rows held in registers over both passes of
+// an append 55 us with the way back, through shared memory with scalar arithmetic 37 + 21.)
 #include "kernels.hpp"
 #include "launch_utils.cuh"
 #include "mma_utils.cuh"
@@ -124,8 +127,8 @@ struct Run {
     unsigned char *tile; // of the head
 };
 
-// fetch(row, count), then, where the run has a place in the pool, body(run), for every run that begins among the warp's rows [row0, row0 + rows). Rows are read 32 at a time: a run that begins among the first
-// 16 ends among them. seq_ids null: rows are tokens 0, 1, ... of sequence seq_row.
+// fetch(row, count), then, where the run has a place in the pool, body(run), for every run that begins among the warp's rows [row0, row0 + rows). Rows
+// are read 32 at a time: a run that begins among the first 16 ends among them. seq_ids null: rows are tokens 0, 1, ... of sequence seq_row.
 template <typename Fetch, typename Body>
 __device__ __forceinline__ void for_runs(const QuantView &kv, const int32_t *seq_ids, const int32_t *positions, int seq_row, int row0, int rows, int n_rows,
                                          int head, bool skip_none, int32_t *error_flag, Fetch &&fetch, Body &&body) {
