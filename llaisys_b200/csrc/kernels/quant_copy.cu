@@ -127,11 +127,12 @@ struct Run {
     unsigned char *tile; // of the head
 };
 
-// fetch(row, count), then, where the run has a place in the pool, body(run), for every run that begins among the warp's rows [row0, row0 + rows). Rows
-// are read 32 at a time: a run that begins among the first 16 ends among them. seq_ids null: rows are tokens 0, 1, ... of sequence seq_row.
-template <typename Fetch, typename Body>
+// fetch(row, count), then body(run) where the run has a place in the pool and lost() where it has none, for every run that begins among the warp's rows
+// [row0, row0 + rows). Rows are read 32 at a time: a run that begins among the first 16 ends among them. seq_ids null: rows are tokens 0, 1, ... of
+// sequence seq_row.
+template <typename Fetch, typename Body, typename Lost>
 __device__ __forceinline__ void for_runs(const QuantView &kv, const int32_t *seq_ids, const int32_t *positions, int seq_row, int row0, int rows, int n_rows,
-                                         int head, bool skip_none, int32_t *error_flag, Fetch &&fetch, Body &&body) {
+                                         int head, bool skip_none, int32_t *error_flag, Fetch &&fetch, Body &&body, Lost &&lost) {
     const int lane = threadIdx.x & 31;
     const bool in = int64_t(row0) + lane < n_rows;
     const int seq = !in ? -2 : seq_ids ? seq_ids[row0 + lane] : seq_row, pos = !in ? -2 : seq_ids ? positions[row0 + lane] : row0 + lane;
@@ -162,6 +163,7 @@ __device__ __forceinline__ void for_runs(const QuantView &kv, const int32_t *seq
         run.count = __ffs(~behind); // the leader and the rows joined to it
         fetch(run.row, run.count);
         if (!quant_tile_of(kv, its_seq, its_pos / kQuantTokens, error_flag, run.tile)) {
+            lost();
             continue;
         }
         run.tile += int64_t(head) * kv.tile_bytes;
@@ -360,8 +362,10 @@ __global__ void __launch_bounds__(kWarps * 32, 8) quant_append_kernel(QuantView 
         } else {
             all ? append_run<T, kF8, false, true>(kv, run, smem) : append_run<T, kF8, false, false>(kv, run, smem);
         }
+    }, [] { // the rows are on their way to where the next run's will lie: copies have no order among themselves
+        cp_async_wait<0>();
+        __syncwarp();
     });
-    cp_async_wait<0>(); // (of runs that have no place)
 }
 
 template <typename T, bool kF8, int kVecs, bool kV, bool kAll>
@@ -438,7 +442,7 @@ __global__ void __launch_bounds__(kWarps * 32, kVecs > 4 ? 6 : 10) quant_gather_
             all ? gather_run<T, kF8, kVecs, false, true>(kv, run, rows, row_step, s_turn[warp])
                 : gather_run<T, kF8, kVecs, false, false>(kv, run, rows, row_step, s_turn[warp]);
         }
-    });
+    }, [] {});
 }
 
 // body(T{}, kF8, kVecs)

@@ -255,6 +255,42 @@ def test_append_skips_rows_without_sequence_and_flags_bad_ones(cuda_device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,store,nkvh,d", [("bf16", "i8", 4, 128), ("f16", "f8", 8, 64), ("f32", "i8", 4, 96), ("bf16", "f8", 3, 256)])
+def test_append_of_many_rows_among_them_some_without_a_place(cuda_device, dtype, store, nkvh, d):
+    """Runs that are skipped or flagged between runs that are stored, several to a warp: the others are what they are without them."""
+    rng = np.random.default_rng(nkvh)
+    lens = rng.integers(0, 60, 90)
+    f = Filled(lens.tolist(), nkvh, d, dtype, store, extra=40)
+    seq, pos, good = [], [], []
+    for i, held in enumerate(lens.tolist()):
+        n = int(rng.integers(1, 40))
+        good.append((i, held, n, len(seq)))
+        seq += [f.seqs[i]] * n
+        pos += range(held, held + n)
+        for _ in range(int(rng.integers(1, 3))):
+            m = int(rng.integers(1, 20))
+            at, s = [(0, 99), (1 << 20, f.seqs[i]), (7, -1), (-1, -1), (3, 1 << 30)][int(rng.integers(0, 5))]
+            seq += [s] * m
+            pos += [at] * m if at < 0 else range(at, at + m)
+    rows = len(seq)
+    assert rows * 2 * nkvh > 64 * torch.cuda.get_device_properties(0).multi_processor_count  # the form of many rows
+    k, v = f.rows(rows), f.rows(rows)
+    bad = torch.ones(rows, dtype=torch.bool)
+    for _, _, n, at in good:
+        bad[at:at + n] = False
+    k[bad] *= 1000  # what would be seen anywhere else
+    v[bad] *= 1000
+    f.cache.append_dev(0, k.cuda(), v.cuda(), i32(seq), i32(pos), rows, stream())
+    for i, held, n, at in good:
+        f.k[i].append(held, k[at:at + n].float().numpy())
+        f.v[i].append(held, v[at:at + n].float().numpy())
+    with pytest.raises(llaisys.LlaisysError) as e:
+        f.cache.check()
+    assert e.value.status == Status.KERNEL
+    f.check_rows()
+
+
+@pytest.mark.gpu
 def test_host_forms_fork_and_prefix(cuda_device):
     f = Filled([37, 5], 2, 64, "f16", "i8", 16, extra=20)
     k, v = f.rows(4), f.rows(4)
