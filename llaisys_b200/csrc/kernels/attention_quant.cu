@@ -718,6 +718,7 @@ __global__ void __launch_bounds__(Shape<D, R>::kThreads, Shape<D, R>::kCtas) att
                     for (int at = 16 * lane; at < tile_bytes; at += 512) {
                         *reinterpret_cast<uint4 *>(my_ring + slot[b] * S::kTile + at) = make_uint4(0, 0, 0, 0);
                     }
+                    fence_proxy_async_smem(); // before the slot's next copy
                     __syncwarp();
                 }
                 whole = whole && live[b] && token0[b] <= whole_to && (token0[b] >= whole_from || token0[b] + kQuantTokens <= p.keep_first);

@@ -437,6 +437,35 @@ def test_rows_that_see_nothing_and_lost_blocks(cuda_device, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,nh,nkvh,d,store", [("bf16", 12, 2, 128, "i8"), ("f16", 32, 8, 64, "f8"), ("f32", 8, 2, 96, "i8"), ("bf16", 20, 1, 256, "f8")])
+@pytest.mark.parametrize("window", [0, 50])
+def test_sequences_that_do_not_exist_beside_others(cuda_device, dtype, nh, nkvh, d, store, window):
+    """Queries of no sequence between others: flagged, and the others' answers are what they are without them."""
+    lens = [1, 70, 333, 16, 900, 45, 2050, 300]
+    f = Filled(lens, nkvh, d, dtype, store)
+    ids = [x for s in f.seqs for x in (s, 99)]
+    for count in (1, 5):  # single queries; chunks
+        kv = [x for n in lens for x in (max(n, count), 700)]
+        q = torch.randn(len(ids) * count, nh, d, generator=torch.Generator().manual_seed(5)).to(TORCH[dtype])
+        qd, out = q.cuda(), torch.full((len(ids) * count, nh, d), 9.0, dtype=TORCH[dtype], device="cuda")
+        starts = i32(range(0, len(ids) * count + 1, count)) if count > 1 else None
+        f.cache.attention_dev(0, out, qd, i32(ids), starts, i32(kv), n_seqs=len(ids), total_q=len(ids) * count, max_q_len=count, max_kv_len=2050, nh=nh,
+                              scale=d ** -0.5, stream=stream(), window=window)
+        assert f.cache.last_kernel() == llaisys.Kernel.EIGHT_BIT
+        got = out.cpu().view(len(ids), count, nh, d).double()
+        assert (got[1::2] == 0).all()
+        for i, n in enumerate(lens):
+            if n < count:
+                continue
+            k, v = (torch.from_numpy(x.worth()).double() for x in (f.k[i], f.v[i]))
+            want, top, big = attention_f64(q[2 * i * count:(2 * i + 1) * count].double(), k, v, n - count, d ** -0.5, window)
+            assert ((got[2 * i] - want).abs() <= tolerance(want, top, big, dtype, n, d)).all(), (count, i)
+        with pytest.raises(llaisys.LlaisysError) as e:
+            f.cache.check()
+        assert e.value.status == Status.KERNEL
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype,nh,nkvh,d", [("bf16", 2, 2, 128), ("f16", 4, 1, 64), ("f32", 12, 2, 96), ("bf16", 16, 1, 256)])
 def test_tables_that_are_full(cuda_device, dtype, nh, nkvh, d):
     """Sequences that end in the last block of their tables: nothing behind it is looked up."""
