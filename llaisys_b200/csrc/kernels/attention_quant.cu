@@ -413,11 +413,12 @@ __global__ void __launch_bounds__(Shape<D, R>::kThreads, Shape<D, R>::kCtas) att
             }
             mbar_init_fence();
         }
-        // (launched programmatically: all but the set-up waits for the kernel in front; with overlap its index arrays are older than that kernel)
+        // (launched programmatically: all but the set-up waits for the kernel in front; with overlap its index arrays are older than that kernel. The kernel
+        // behind is let go only when the one in front has ended, whose results it may then count on without a wait of its own.)
         if (!p.overlap) {
             grid_dependency_wait();
+            grid_launch_dependents();
         }
-        grid_launch_dependents();
         int64_t *sums = reinterpret_cast<int64_t *>(s_merge);
         const int per = (p.n_seqs + kThreads - 1) / kThreads, a0 = min(tid * per, p.n_seqs), a1 = min(a0 + per, p.n_seqs);
         int64_t mine = 0;
@@ -574,6 +575,7 @@ __global__ void __launch_bounds__(Shape<D, R>::kThreads, Shape<D, R>::kCtas) att
     feed.count = 0;
     if (p.overlap) {
         grid_dependency_wait();
+        grid_launch_dependents();
     }
     more = step();
     __syncthreads(); // the sums' place is the queries'

@@ -665,6 +665,41 @@ def test_steps_with_launch_overlap(cuda_device, dtype, nh, d):
 
 
 @pytest.mark.gpu
+def test_launch_overlap_of_two_caches(cuda_device):
+    """Rows appended to a 16-bit cache, attention of an 8-bit one, decode of the first: with overlap the decode reads older pages ahead of its own wait,
+    because the kernel in front of it was let go behind the append."""
+    n, held, d, nh = 16, 2048, 128, 8
+    f = Filled([300] * 8, 2, d, "bf16", "i8")
+    pages = held // 16
+    cache = llaisys.PagedKVCache(n * pages, 2, d, dtype=llaisys.DataType.BF16, device=llaisys.DeviceType.NVIDIA, max_seqs=n, max_pages_per_seq=pages)
+    seqs = [cache.add_seq() for _ in range(n)]
+    for i, s in enumerate(seqs):
+        cache.assign_pages(s, range(i * pages, (i + 1) * pages))
+    cache.flush()
+    g = torch.Generator().manual_seed(1)
+    rows = [[torch.randn(n * held, 2, d, generator=g).bfloat16().cuda() for _ in range(2)] for _ in range(3)]
+    q8, q16 = torch.randn(8, nh, d, generator=g).bfloat16().cuda(), torch.randn(n, nh, d, generator=g).bfloat16().cuda()
+    ids8, kv8, ids, kv = i32(f.seqs), i32([300] * 8), i32(seqs), i32([held] * n)
+    seq, pos = i32(np.repeat(seqs, held)), i32(np.tile(np.arange(held), n))
+    outs = []
+    for overlap in (False, True):
+        out8, out16 = (torch.zeros(3, *q.shape, dtype=q.dtype, device="cuda") for q in (q8, q16))
+        torch.cuda.synchronize()
+        cache.set_launch_overlap(overlap)
+        f.cache.set_launch_overlap(overlap)
+        for i, (k, v) in enumerate(rows):  # (the pages hold the turn before's rows until the append is through)
+            cache.append_dev(0, k, v, seq, pos, n * held, stream())
+            f.cache.decode_dev(0, out8[i], q8, ids8, kv8, 8, 300, nh, 0.1, stream())
+            cache.decode_dev(0, out16[i], q16, ids, kv, n, held, nh, 0.1, stream())
+        torch.cuda.synchronize()
+        cache.check()
+        f.cache.check()
+        outs.append((out8.cpu(), out16.cpu()))
+    for a, b in zip(*outs):
+        assert torch.equal(a, b) and a.abs().max() > 0
+
+
+@pytest.mark.gpu
 def test_two_caches_on_two_streams_and_graphs(cuda_device):
     """Calls of two caches side by side, eager and replayed, give what they give alone."""
     sides = []
