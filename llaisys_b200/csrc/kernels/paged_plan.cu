@@ -216,20 +216,18 @@ __global__ void __launch_bounds__(kThreads) paged_plan_kernel(PlanArgs p) {
                 entry = -1;
             }
             const int pos = q.held + int(r - start);
+            const int e = p.table == nullptr ? 0 : p.page_shift >= 0 ? pos >> p.page_shift : pos / p.page_size;
+            const bool in_table = q.row >= 0 && e < p.table_stride, read = e < q.held_pages || p.free_pages == nullptr;
+            if (p.table != nullptr && !(in_table && (read || (enough && q.grown > 0)))) {
+                continue; // no page: what the table holds there is not this request's, so nothing is to be appended through it
+            }
             seqs[k] = p.seq_ids ? p.seq_ids[i] : i;
             positions[k] = pos;
             if (p.row_slots != nullptr) {
-                const int e = p.page_shift >= 0 ? pos >> p.page_shift : pos / p.page_size;
                 if (e != entry) {
                     entry = e;
-                    page = -1;
-                    if (q.row >= 0 && e < p.table_stride) {
-                        if (e < q.held_pages || p.free_pages == nullptr) {
-                            page = p.table[int64_t(q.row) * p.table_stride + e];
-                        } else if (enough && q.grown > 0) {
-                            page = p.free_pages[grown + e - q.held_pages]; // (its entry may be another CTA's to write)
-                        }
-                    }
+                    // (a new page's entry may be another CTA's to write)
+                    page = read ? p.table[int64_t(q.row) * p.table_stride + e] : p.free_pages[grown + e - q.held_pages];
                 }
                 slots[k] = page < 0 ? -1 : int64_t(page) * p.page_size + (pos - e * p.page_size);
             }

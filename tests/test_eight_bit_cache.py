@@ -580,6 +580,48 @@ def test_plan_what_cannot_be_done(cuda_device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("free,new,flags", [([], [20, 14, 7, 30, 8], 1), ([11, 12, 13], [20, 14, 7, 30, 8], 1), ([11, 12, 13, 14], [20, 30, 7, 30, 8], 8),
+                                            ([11, 12, 13], [20, 30, 7, 30, 8], 9)])
+@pytest.mark.parametrize("slots", [False, True])
+def test_plan_rows_without_a_page_are_not_appended(cuda_device, free, new, flags, slots):
+    """Too few free pages, a request longer than its row of the table: the step's append leaves alone what the entries behind the requests' pages name."""
+    lens = [20, 33, 16, 5, 40]
+    f = Filled(lens, 2, 64, "bf16", "i8")
+    stride, total = max(f.room), sum(new)
+    table = np.zeros((len(lens) + 2, stride), np.int32)  # as the cache's: page 0 behind a sequence's last one
+    for s, n in zip(f.seqs, f.room):
+        table[s, :n] = f.cache.seq_pages(s)
+    t, fr = torch.from_numpy(table).cuda(), i32(free + [0])
+    seqs, pos = (torch.full((total + 5,), 7, dtype=torch.int32, device="cuda") for _ in range(2))
+    status, at = i32([9, 9]), torch.full((total + 5,), 7, dtype=torch.int64, device="cuda")
+    ids, hd, nd = i32(f.seqs), i32(lens), i32(new)
+    llaisys.paged_plan_dev(stream=stream(), seq_ids_dev=ids, held_dev=hd, new_dev=nd, n_seqs=len(lens), page_size=16, n_rows=total + 5, free_pages_dev=fr,
+                           n_free=len(free), block_table_dev=t, table_rows=len(table), table_stride=stride, row_seqs_dev=seqs, row_positions_dev=pos,
+                           row_slots_dev=at if slots else None, status_dev=status)
+    k, v = f.rows(total + 5), f.rows(total + 5)
+    grown = flags == 8
+    assert status.tolist() == [4 if grown else 0, flags]
+    want_seqs, want_pos, row = [], [], 0
+    for i, (s, held, n) in enumerate(zip(f.seqs, lens, new)):
+        room = 16 * (stride if grown and held + n <= 16 * stride else f.room[i])
+        kept = min(n, room - held)
+        want_seqs += [s] * kept + [-1] * (n - kept)
+        want_pos += [*range(held, held + kept)] + [-1] * (n - kept)
+        kept = min(n, 16 * f.room[i] - held)  # (the cache's own table has none of the new pages)
+        f.k[i].append(held, k[row:row + kept].float().numpy())
+        f.v[i].append(held, v[row:row + kept].float().numpy())
+        row += n
+    assert seqs.tolist() == want_seqs + [-1] * 5 and pos.tolist() == want_pos + [-1] * 5
+    if slots:
+        assert ((at < 0) == (seqs < 0)).all()
+    if grown:
+        return
+    f.cache.append_dev(0, k.cuda(), v.cuda(), seqs, pos, total + 5, stream())
+    f.cache.check()
+    f.check_rows()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype,store", [("bf16", "i8"), ("f32", "f8")])
 def test_steps_planned_on_the_gpu_and_replayed(cuda_device, dtype, store):
     """Plan, append and attention of a few steps, nothing read back in between; the last form captured once and replayed with other lengths."""
