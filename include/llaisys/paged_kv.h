@@ -272,10 +272,11 @@ LLAISYS_API int llaisysPagedAttentionPrefillDev(llaisysPagedKV_t kv, size_t laye
  *   status_dev [2]                pages taken, and LLAISYS_PLAN_ bits
  * Any output may be NULL, and so may the table when neither slots nor growth are wanted; no output lies over an input. Rows behind the last request's, up to n_rows, are -1
  * (such rows are skipped by appends to a cache held in 8 bits). A request may appear once.
- * What cannot be done is left out and flagged, never written elsewhere: too few free pages take none at all; rows behind n_rows are dropped (q_starts
- * ends at n_rows); negative counts and sums over 2^31 - 1 count as nothing brought; a request whose row or last page lies outside the table gets no
- * page. Rows that have no page for these reasons are -1 in all three arrays, so that an append skips them too; q_starts and kv_lens count them all
- * the same, and what attention makes of such a request is of no use: the entries behind its pages are not its own. */
+ * What cannot be done is left out and flagged, never written elsewhere: rows behind n_rows count as not brought, in every array (the requests they
+ * belong to may bring them in a later step); too few free pages take none at all; negative counts and sums over 2^31 - 1 count as nothing brought; a
+ * request whose row or last page lies outside the table gets no page. Rows that have no page for these reasons are -1 in all three arrays, so that
+ * an append skips them too; q_starts and kv_lens count them all the same, and what attention makes of such a request is of no use: the entries behind
+ * its pages are not its own. */
 #define LLAISYS_PLAN_NO_PAGES 1
 #define LLAISYS_PLAN_ROWS_DROPPED 2
 #define LLAISYS_PLAN_BAD_COUNT 4

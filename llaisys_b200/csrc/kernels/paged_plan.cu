@@ -30,7 +30,8 @@ __device__ __forceinline__ int pages_of(int tokens, const PlanArgs &p) {
     return p.page_shift >= 0 ? int((uint32_t(tokens) + uint32_t(p.page_size) - 1u) >> p.page_shift)
                              : int((uint32_t(tokens) + uint32_t(p.page_size) - 1u) / uint32_t(p.page_size));
 }
-__device__ __forceinline__ Request load_request(const PlanArgs &p, int i, int &flags) {
+// room: rows there are for it and whoever comes behind it
+__device__ __forceinline__ Request load_request(const PlanArgs &p, int i, int room, int &flags) {
     Request q;
     q.row = p.seq_ids ? p.seq_ids[i] : i;
     q.held = p.held[i];
@@ -40,6 +41,7 @@ __device__ __forceinline__ Request load_request(const PlanArgs &p, int i, int &f
         q.held = max(q.held, 0);
         q.fresh = 0;
     }
+    q.fresh = min(q.fresh, room);
     if (p.table != nullptr && (q.row < 0 || q.row >= p.table_rows)) {
         flags |= LLAISYS_PLAN_BAD_ROW;
         q.row = -1;
@@ -58,8 +60,8 @@ __device__ __forceinline__ Request load_request(const PlanArgs &p, int i, int &f
 }
 
 // The last chunk whose sum in front is not over x (chunks that add nothing in front of it are passed over).
-template <int kChunks, typename T>
-__device__ __forceinline__ int chunk_of(const T *sums, int64_t x) {
+template <int kChunks>
+__device__ __forceinline__ int chunk_of(const int *sums, int x) {
     int lo = 0, hi = kChunks - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
@@ -76,7 +78,7 @@ template <int kThreads>
 __global__ void __launch_bounds__(kThreads) paged_plan_kernel(PlanArgs p) {
     constexpr int kWarps = kThreads / 32;
     __shared__ int64_t s_warp[kWarps][3];
-    __shared__ int64_t s_rows[kThreads]; // rows in front of a chunk
+    __shared__ int s_rows[kThreads];     // rows in front of a chunk
     __shared__ int s_grown[kThreads];    // pages taken in front of it
     __shared__ int s_flags;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -85,66 +87,85 @@ __global__ void __launch_bounds__(kThreads) paged_plan_kernel(PlanArgs p) {
     }
     const int per = int((int64_t(p.n_seqs) + kThreads - 1) / kThreads), i0 = int(min(int64_t(tid) * per, int64_t(p.n_seqs)));
     const int i1 = i0 + min(per, p.n_seqs - i0);
-    int flags = 0;
-    int64_t mine[3] = {0, 0, 0}; // rows, pages, pages taken
-    for (int i = i0; i < i1; ++i) {
-        const Request q = load_request(p, i, flags);
-        mine[0] += q.fresh;
-        mine[1] += q.pages;
-        mine[2] += q.grown;
-    }
-    int64_t before[3] = {mine[0], mine[1], mine[2]};
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-#pragma unroll
-        for (int k = 0; k < 3; ++k) {
-            const int64_t up = __shfl_up_sync(0xffffffffu, before[k], o);
-            before[k] += lane >= o ? up : 0;
+    int flags;
+    int64_t mine[3], before[3], total[3]; // rows, pages, pages taken: of this thread's chunk, in front of it, of all
+    bool dropped = false;
+    for (;;) {
+        int64_t front = dropped ? min(before[0], int64_t(p.n_rows)) : 0;
+        flags = 0;
+        mine[0] = mine[1] = mine[2] = 0;
+        for (int i = i0; i < i1; ++i) {
+            const Request q = load_request(p, i, dropped ? int(p.n_rows - front) : INT_MAX, flags);
+            front += q.fresh;
+            mine[0] += q.fresh;
+            mine[1] += q.pages;
+            mine[2] += q.grown;
         }
-    }
-    if (lane == 31) {
 #pragma unroll
         for (int k = 0; k < 3; ++k) {
-            s_warp[warp][k] = before[k];
+            before[k] = mine[k];
         }
-    }
-    __syncthreads();
-    if (flags != 0) {
-        atomicOr(&s_flags, flags);
-    }
-    if (warp == 0) {
 #pragma unroll
-        for (int k = 0; k < 3; ++k) {
-            int64_t v = lane < kWarps ? s_warp[lane][k] : 0;
+        for (int o = 1; o < 32; o <<= 1) {
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int64_t up = __shfl_up_sync(0xffffffffu, v, o);
-                v += lane >= o ? up : 0;
-            }
-            if (lane < kWarps) {
-                s_warp[lane][k] = v;
+            for (int k = 0; k < 3; ++k) {
+                const int64_t up = __shfl_up_sync(0xffffffffu, before[k], o);
+                before[k] += lane >= o ? up : 0;
             }
         }
-    }
-    __syncthreads();
-    int64_t total[3];
+        if (lane == 31) {
 #pragma unroll
-    for (int k = 0; k < 3; ++k) {
-        before[k] += (warp > 0 ? s_warp[warp - 1][k] : 0) - mine[k];
-        total[k] = s_warp[kWarps - 1][k];
+            for (int k = 0; k < 3; ++k) {
+                s_warp[warp][k] = before[k];
+            }
+        }
+        __syncthreads();
+        if (flags != 0) {
+            atomicOr(&s_flags, flags);
+        }
+        if (warp == 0) {
+#pragma unroll
+            for (int k = 0; k < 3; ++k) {
+                int64_t v = lane < kWarps ? s_warp[lane][k] : 0;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int64_t up = __shfl_up_sync(0xffffffffu, v, o);
+                    v += lane >= o ? up : 0;
+                }
+                if (lane < kWarps) {
+                    s_warp[lane][k] = v;
+                }
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+            before[k] += (warp > 0 ? s_warp[warp - 1][k] : 0) - mine[k];
+            total[k] = s_warp[kWarps - 1][k];
+        }
+        if (dropped || total[0] <= p.n_rows) {
+            break;
+        }
+        // More rows than there is room for: once more, without what is dropped, which then counts as not brought in lengths and pages too.
+        dropped = true;
+        __syncthreads();
+        if (tid == 0) {
+            s_flags = 0;
+        }
     }
     const bool enough = total[2] <= p.n_free;
-    s_rows[tid] = before[0];
+    s_rows[tid] = int(before[0]); // (n_rows at most by now)
     s_grown[tid] = int(min(before[2], int64_t(INT_MAX)));
     __syncthreads();
 
     // ---- this CTA's share of the requests, by warps: what is said about each
     if (warp * int(gridDim.x) / kWarps == int(blockIdx.x)) {
-        int64_t rows = before[0], pages = before[1];
+        int rows = int(before[0]);
+        int64_t pages = before[1];
         for (int i = i0; i < i1; ++i) {
-            const Request q = load_request(p, i, flags);
+            const Request q = load_request(p, i, p.n_rows - rows, flags);
             if (p.q_starts) {
-                p.q_starts[i] = int(min(rows, int64_t(p.n_rows)));
+                p.q_starts[i] = rows;
             }
             if (p.kv_lens) {
                 p.kv_lens[i] = q.held + q.fresh;
@@ -159,26 +180,28 @@ __global__ void __launch_bounds__(kThreads) paged_plan_kernel(PlanArgs p) {
     // ---- its share of the new entries of the table
     if (enough) {
         for (int64_t e = int64_t(blockIdx.x) * kThreads + tid; e < total[2]; e += int64_t(gridDim.x) * kThreads) {
-            const int chunk = chunk_of<kThreads>(s_grown, e);
+            const int chunk = chunk_of<kThreads>(s_grown, int(e));
             int i = chunk * per, first = s_grown[chunk];
-            Request q = load_request(p, i, flags);
+            int rows = s_rows[chunk];
+            Request q = load_request(p, i, p.n_rows - rows, flags);
             while (e >= first + q.grown) {
                 first += q.grown;
-                q = load_request(p, ++i, flags);
+                rows += q.fresh;
+                q = load_request(p, ++i, p.n_rows - rows, flags);
             }
             p.table[int64_t(q.row) * p.table_stride + q.held_pages + (e - first)] = p.free_pages[e];
         }
     }
     if (blockIdx.x == 0 && tid == 0) {
         if (p.q_starts) {
-            p.q_starts[p.n_seqs] = int(min(total[0], int64_t(p.n_rows)));
+            p.q_starts[p.n_seqs] = int(total[0]);
         }
         if (p.page_starts) {
             p.page_starts[p.n_seqs] = int(min(total[1], int64_t(INT_MAX)));
         }
         if (p.status) {
             p.status[0] = enough ? int(total[2]) : 0;
-            p.status[1] = s_flags | (enough ? 0 : LLAISYS_PLAN_NO_PAGES) | (total[0] > p.n_rows ? LLAISYS_PLAN_ROWS_DROPPED : 0);
+            p.status[1] = s_flags | (enough ? 0 : LLAISYS_PLAN_NO_PAGES) | (dropped ? LLAISYS_PLAN_ROWS_DROPPED : 0);
         }
     }
 
@@ -186,13 +209,13 @@ __global__ void __launch_bounds__(kThreads) paged_plan_kernel(PlanArgs p) {
     if (p.row_seqs == nullptr && p.row_positions == nullptr && p.row_slots == nullptr) {
         return;
     }
-    const int live = int(min(total[0], int64_t(p.n_rows)));
+    const int live = int(total[0]);
     for (int64_t r0 = (int64_t(blockIdx.x) * kThreads + tid) * kRowsAtOnce; r0 < p.n_rows; r0 += int64_t(gridDim.x) * kThreads * kRowsAtOnce) {
         int seqs[kRowsAtOnce], positions[kRowsAtOnce];
         int64_t slots[kRowsAtOnce];
-        const int lo = r0 < live ? chunk_of<kThreads>(s_rows, r0) : 0;
+        const int lo = r0 < live ? chunk_of<kThreads>(s_rows, int(r0)) : 0;
         int i = lo * per;
-        int64_t start = s_rows[lo];
+        int start = s_rows[lo];
         int grown = s_grown[lo];
         Request q{};
         int entry = -1, page = -1; // the entry of the table that `page` is from
@@ -211,7 +234,7 @@ __global__ void __launch_bounds__(kThreads) paged_plan_kernel(PlanArgs p) {
                     grown += q.grown;
                     ++i;
                 }
-                q = load_request(p, i, flags);
+                q = load_request(p, i, p.n_rows - start, flags);
                 loaded = true;
                 entry = -1;
             }

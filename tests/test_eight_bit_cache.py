@@ -622,6 +622,28 @@ def test_plan_rows_without_a_page_are_not_appended(cuda_device, free, new, flags
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n,high,long,page", [(3, 40, 30, 16), (64, 300, 9, 16), (700, 100, 20, 48), (2500, 50, 60, 32)])
+@pytest.mark.parametrize("room", [0, 1, 0.37, 0.98])
+def test_plan_of_more_rows_than_there_is_room_for(cuda_device, n, high, long, page, room):
+    """Dropped rows are rows that were not brought: lengths, pages and growth agree with the rows that are left."""
+    rng = np.random.default_rng(n)
+    held, new = rng.integers(0, high + 1, n), rng.integers(0, long + 1, n)
+    rows = room if isinstance(room, int) else int(new.sum() * room)
+    front = np.concatenate([[0], np.cumsum(new)[:-1]])
+    kept = np.clip(rows - front, 0, new)
+    stride = max(1, int((-(-(held + kept) // page)).max()))  # (what is dropped need not fit the table)
+    ids = rng.permutation(n + 3)[:n]
+    table = rng.integers(0, 9999, (n + 3, stride)).astype(np.int32)
+    free = rng.permutation(int((-(-(held + kept) // page) + -held // page).sum())).astype(np.int32)  # nor be paid in pages
+    got, t = run_plan(ids, held, new, page, rows, free, table)
+    want, w = plan_reference(ids.tolist(), held.tolist(), kept.tolist(), page, rows, free, table)
+    want["status"][1] = 2
+    for key, value in want.items():
+        assert np.array_equal(got[key], value), key
+    assert np.array_equal(t, w)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype,store", [("bf16", "i8"), ("f32", "f8")])
 def test_steps_planned_on_the_gpu_and_replayed(cuda_device, dtype, store):
     """Plan, append and attention of a few steps, nothing read back in between; the last form captured once and replayed with other lengths."""
