@@ -49,10 +49,10 @@ __device__ __forceinline__ Request load_request(const PlanArgs &p, int i, int ro
     q.held_pages = pages_of(q.held, p);
     q.pages = pages_of(q.held + q.fresh, p);
     q.grown = 0;
-    if (p.free_pages != nullptr && q.row >= 0 && q.fresh > 0) {
+    if (p.table != nullptr && q.row >= 0 && q.fresh > 0) {
         if (q.pages > p.table_stride) {
             flags |= LLAISYS_PLAN_BAD_ROW;
-        } else {
+        } else if (p.free_pages != nullptr) {
             q.grown = q.pages - q.held_pages;
         }
     }

@@ -644,6 +644,19 @@ def test_plan_of_more_rows_than_there_is_room_for(cuda_device, n, high, long, pa
 
 
 @pytest.mark.gpu
+def test_plan_with_a_table_that_is_only_read_flags_requests_outside_it(cuda_device):
+    table = np.arange(40, dtype=np.int32).reshape(4, 10)
+    got, t = run_plan([1, 3], [150, 20], [20, 3], 16, 24, None, table)
+    assert got["status"].tolist() == [0, 8] and np.array_equal(t, table)
+    assert got["row_slots"].tolist() == [19 * 16 + 6 + i for i in range(10)] + [-1] * 10 + [31 * 16 + 4 + i for i in range(3)] + [-1]
+    assert got["row_seqs"].tolist() == [1] * 10 + [-1] * 10 + [3] * 3 + [-1]
+    got, _ = run_plan([1, 3], [150, 20], [10, 3], 16, 24, None, table)  # to the row's end
+    assert got["status"].tolist() == [0, 0]
+    got, _ = run_plan([1, 9], [150, 20], [10, 3], 16, 24, None, table)
+    assert got["status"].tolist() == [0, 8] and (got["row_seqs"][10:] == -1).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype,store", [("bf16", "i8"), ("f32", "f8")])
 def test_steps_planned_on_the_gpu_and_replayed(cuda_device, dtype, store):
     """Plan, append and attention of a few steps, nothing read back in between; the last form captured once and replayed with other lengths."""
