@@ -42,6 +42,9 @@ constexpr uint32_t kWaitLimit = 1u << 20;
 constexpr int kErrTimeout = 8;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kShift = 14.f; // weights are 2^14 times what they stand for
+// Smallest power of two taken out of a V scale. A row's sum has 2^14 2^-e for a token of the largest weight: 2^31 tokens of the smallest scale (values
+// all zero, say) stay below 2^128. What is left of scales below 2^-82 is in the weights, of which the f16 numbers then carry fewer bits below the largest.
+constexpr int kLeastPower = -82;
 constexpr size_t kPlaceBytes = 512;
 
 // Heads of up to 128: two CTAs of four warps on an SM, each warp with two blocks at a time and 255 registers. Longer ones: one CTA of eight warps.
@@ -804,7 +807,7 @@ __global__ void __launch_bounds__(Shape<D, R>::kThreads, Shape<D, R>::kCtas) att
                         x = fmaf(x, by, less);
                     }
                 }
-                const int e = max(-100, min(126, ((__float_as_int(scales.y) >> 23) & 255) - 127));
+                const int e = max(kLeastPower, min(126, ((__float_as_int(scales.y) >> 23) & 255) - 127));
                 fe[b] = float(e);
                 down[b] = power_of_two(-e);
                 mantissa[b] = scales.y * down[b];

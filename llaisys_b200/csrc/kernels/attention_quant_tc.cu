@@ -45,6 +45,8 @@ static_assert(sizeof(Place) <= kPlaceInts * sizeof(int), "a warp's words");
 constexpr int kErrTimeout = 8;
 constexpr float kRescaleThreshold = 8.f; // log2 units
 constexpr float kShift = 7.f;            // weights are 2^7 times what they stand for: at most 2^15 with a maximum that lags by the threshold
+// A row's sum is kept as 2^-18 of itself: it has 2^15 / s_v for a token, and 2^30 tokens of the smallest scale, 2^-100 (values all zero, say), stay below 2^128.
+constexpr float kSumUnit = 0x1p-18f;
 constexpr int kFeedSlots = 4;            // blocks whose tiles the guide has found ahead of the operand warps
 constexpr int kPlaces = 11;              // warps that keep a place on the line: all but the operand warps and the last one
 constexpr int kScaleSlots = 4;           // blocks whose scales are kept: a block's slot is written again when its turn has passed twice over
@@ -147,7 +149,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_quant_tc_kernel(QuantCh
         return;
     }
     const uint32_t ring_u32 = base_u32 + 2 * kQBytes;
-    float4 *s_scales = reinterpret_cast<float4 *>(base + S::kScales); // [slot][block of 16 keys]: s_k, log2 s_v, 1 / s_v
+    float4 *s_scales = reinterpret_cast<float4 *>(base + S::kScales); // [slot][block of 16 keys]: s_k, log2 s_v, kSumUnit / s_v
     signed char *s_power = reinterpret_cast<signed char *>(base + S::kFactors); // [fragments in turn][row of the tile]: raw scores are 2^-power of what they stand for
     uint64_t *bars = reinterpret_cast<uint64_t *>(base + S::kBarsAt);
     const uint32_t bars_u32 = smem_u32(bars);
@@ -497,7 +499,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_quant_tc_kernel(QuantCh
                     // (a block never written to has no scale; the NaN of a lost one is in the logarithm, and so in the weights of whoever sees it, and not in
                     // what the sums of all others are multiplied by)
                     const float s_v = s_feed[b].s_v < kQuantFloor ? kQuantFloor : s_feed[b].s_v;
-                    s_scales[heard % kScaleSlots * kPagesPerBlock + block_a + 2 * lane] = make_float4(s_feed[b].s_k, fast_log2(s_v), isnan(s_v) ? 0.f : 1.f / s_v, 0.f);
+                    s_scales[heard % kScaleSlots * kPagesPerBlock + block_a + 2 * lane] = make_float4(s_feed[b].s_k, fast_log2(s_v), isnan(s_v) ? 0.f : kSumUnit / s_v, 0.f);
                 }
                 __syncwarp();
                 if (lane == 0) {
@@ -918,7 +920,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_quant_tc_kernel(QuantCh
                 }
             }
             if (store_rows && !dead) {
-                float inv = l_all > 0.f ? 1.f / l_all : 0.f;
+                float inv = l_all > 0.f ? kSumUnit / l_all : 0.f;
                 if (p.row_scale != nullptr && t < g.q_len) {
                     inv *= p.row_scale[(long long)(g.q_start + t) * p.nh + head];
                 }

@@ -499,6 +499,61 @@ def test_values_of_very_different_size(cuda_device):
     f.check_attention([(0, 60)], 4, chunks=True)
 
 
+def constant_rows(seqs, tokens, nkvh, d, dtype, store, k_of, v_of):
+    """A cache of sequences whose token t has the numbers k_of(t) and v_of(t) in every dim."""
+    pages = -(-tokens // 16)
+    cache = llaisys.PagedKVCache.quantized(seqs * pages, nkvh, d, store=STORES[store], dtype=NAMES[dtype], max_seqs=seqs, max_pages_per_seq=pages)
+    t = torch.arange(tokens, device="cuda")
+    k, v = (of(t).to(TORCH[dtype])[:, None, None].expand(-1, nkvh, d).contiguous() for of in (k_of, v_of))
+    for _ in range(seqs):
+        s = cache.add_seq()
+        cache.reserve(s, tokens)
+        cache.flush()
+        cache.append_dev(0, k, v, torch.full((tokens,), s, dtype=torch.int32, device="cuda"), t.int(), tokens, stream())
+    return cache
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("store", ["i8", "f8"])
+@pytest.mark.parametrize("dtype,nh", [("bf16", 4), ("f32", 4), ("f16", 16)])
+def test_values_that_are_zero_for_long(cuda_device, dtype, store, nh):
+    """20000 tokens of value 0 and equal scores, then 1000 of value 4: the row's sum counts them all."""
+    n, last, d = 21000, 1000, 64
+    cache = constant_rows(1, n, 1, d, dtype, store, lambda t: 0.0 * t, lambda t: 4.0 * (t >= n - last))
+    q = torch.ones(1, nh, d, dtype=TORCH[dtype], device="cuda")
+    out, part = torch.empty_like(q), torch.empty(1, nh, d + 2, device="cuda")
+    # weights are off by 2^-11 (their sum and theirs with the values), the values' code by nothing but the scale's rounding
+    tol = dict(rtol=torch.finfo(TORCH[dtype]).eps / 2 + 2.0 ** -9, atol=0)
+    for held in (n, n - last):
+        value = 4 * last / n if held == n else 0
+        cache.decode_dev(0, out, q, i32([0]), i32([held]), 1, held, nh, 0.1, stream())
+        cache.decode_partial_dev(0, part, q, i32([0]), i32([held]), 1, held, nh, 0.1, stream())
+        assert torch.allclose(out.float().cpu(), torch.tensor(float(value)), **tol)
+        assert torch.allclose(part[..., :d].cpu(), torch.tensor(float(value)), **tol)
+        assert (part[..., d] == 0).all() and torch.allclose(part[..., d + 1].cpu(), torch.tensor(float(held)), rtol=1e-5)
+    cache.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("store", ["i8", "f8"])
+def test_long_chunks_behind_values_that_are_zero_for_long(cuda_device, store):
+    """The same for chunks, a whole tile a CTA, with scores that rise as far as the maximum may lag behind them."""
+    n, rows, d, seqs = 16384, 64, 64, 4
+    nkvh = torch.cuda.get_device_properties(0).multi_processor_count // seqs
+    cache = constant_rows(seqs, n, nkvh, d, "bf16", store, lambda t: 1.0 * (t >= 128), lambda t: 4.0 * (t >= n - 128))
+    q = torch.ones(seqs * rows, 4 * nkvh, d, dtype=torch.bfloat16, device="cuda")
+    out = torch.empty_like(q)
+    rise = 7.9  # a key of ones, in log2 units
+    cache.prefill_dev(0, out, q, i32(range(seqs)), i32(range(0, seqs * rows + 1, rows)), i32([n] * seqs), seqs, seqs * rows, rows, n, 4 * nkvh,
+                      rise * np.log(2) / d, stream())
+    assert cache.last_kernel() == llaisys.Kernel.EIGHT_BIT_TC
+    seen = n - rows + 1 + torch.arange(rows).double()
+    want = 4 * (seen - (n - 128)) * 2 ** rise / ((seen - 128) * 2 ** rise + 128)
+    got = out.view(seqs, rows, -1).cpu().double()
+    assert ((got - want[None, :, None]).abs() <= want[None, :, None] * (2.0 ** -8 + 2.0 ** -9)).all()
+    cache.check()
+
+
 # ---- a step, planned and run ----------------------------------------------------------------------------------------------
 
 
