@@ -376,7 +376,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_quant_tc_kernel(QuantCh
                 const int n = f.b1 - f.b0, seq = p.seq_ids[f.a];
                 const int last = (min(tile_kv_hi(w.g, f.qb), min(max(p.kv_lens[f.a], 0), p.table_stride * kPage)) + kPage - 1) / kPage - 1;
                 const bool known = seq >= 0 && seq < p.kv.table_rows;
-                if (!known) {
+                if (!known && last >= 0) {
                     atomicOr(p.error_flag, kErrBadSeq);
                 }
                 const int32_t *table = p.kv.block_table + (long long)(known ? seq : 0) * p.kv.table_stride;
@@ -497,9 +497,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_quant_tc_kernel(QuantCh
                 if (lane < 2) {
                     const int b = heard % kFeedSlots * kPagesPerBlock + block_a + 2 * lane;
                     // (a block never written to has no scale; the NaN of a lost one is in the logarithm, and so in the weights of whoever sees it, and not in
-                    // what the sums of all others are multiplied by)
+                    // what the sums of all others are multiplied by; what has no page is hidden)
                     const float s_v = s_feed[b].s_v < kQuantFloor ? kQuantFloor : s_feed[b].s_v;
-                    s_scales[heard % kScaleSlots * kPagesPerBlock + block_a + 2 * lane] = make_float4(s_feed[b].s_k, fast_log2(s_v), isnan(s_v) ? 0.f : kSumUnit / s_v, 0.f);
+                    s_scales[heard % kScaleSlots * kPagesPerBlock + block_a + 2 * lane] =
+                        make_float4(s_feed[b].s_k, s_feed[b].place < 0 ? -INFINITY : fast_log2(s_v), isnan(s_v) ? 0.f : kSumUnit / s_v, 0.f);
                 }
                 __syncwarp();
                 if (lane == 0) {

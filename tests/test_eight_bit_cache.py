@@ -466,6 +466,56 @@ def test_sequences_that_do_not_exist_beside_others(cuda_device, dtype, nh, nkvh,
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,nh,nkvh,d,page,store", [("bf16", 12, 2, 128, 16, "i8"), ("f16", 32, 8, 64, 32, "f8"), ("f32", 6, 3, 96, 16, "i8"),
+                                                        ("bf16", 16, 1, 128, 64, "f8"), ("f16", 4, 4, 256, 16, "i8")])
+@pytest.mark.parametrize("window", [0, 150])
+def test_pages_that_do_not_exist(cuda_device, dtype, nh, nkvh, d, page, store, window):
+    """Their tokens are nobody's keys, whichever kernel serves the call; so are all tokens of a sequence that does not exist. Both are flagged."""
+    lens = [700, 64, 333, 1029]
+    f = Filled(lens, nkvh, d, dtype, store, page)
+    stride = max(f.room)
+    lost = [[0, 3, 4, 10], [], [f.room[2] - 1], list(range(f.room[3] // 2, f.room[3] - 1))]
+    table = np.zeros((len(lens) + 2, stride), np.int32)
+    for s, pages, gone in zip(f.seqs, f.room, lost):
+        table[s, :pages] = f.cache.seq_pages(s)
+        table[s, [e for e in gone if e < pages]] = -1 if s % 2 else 1 << 20
+    torch.cuda.synchronize()
+    llaisys.RuntimeAPI(llaisys.DeviceType.NVIDIA).memcpy_sync(f.cache.block_table_ptr(), table.ctypes.data, table.nbytes, llaisys.MemcpyKind.H2D)
+    ids = [*f.seqs, 77]
+    for counts, tc in (([1] * 5, False), ([3, 1, 5, 2, 4], False), ([300, 64, 200, 513, 90], d in (64, 128) and dtype != "f32")):
+        starts, total = np.concatenate([[0], np.cumsum(counts)]), sum(counts)
+        q = torch.randn(total, nh, d, generator=torch.Generator().manual_seed(5)).to(TORCH[dtype])
+        qd, out = q.cuda(), torch.full((total, nh, d), 9.0, dtype=TORCH[dtype], device="cuda")
+        f.cache.attention_dev(0, out, qd, i32(ids), i32(starts) if total > 5 else None, i32([*lens, 500]), n_seqs=5, total_q=total, max_q_len=max(counts),
+                              max_kv_len=max(lens), nh=nh, scale=d ** -0.5, stream=stream(), window=window)
+        assert (f.cache.last_kernel() == llaisys.Kernel.EIGHT_BIT_TC) == tc
+        got = out.cpu().double()
+        assert (got[starts[4]:] == 0).all()
+        for i, n in enumerate(lens):
+            rows = slice(starts[i], starts[i + 1])
+            k, v = (torch.from_numpy(x.worth()).double().repeat_interleave(nh // nkvh, 1) for x in (f.k[i], f.v[i]))
+            t, j = torch.arange(n - counts[i], n)[:, None], torch.arange(n)[None]
+            seen = (j <= t) & (t - j < (window or n)) & ~torch.isin(j // page, torch.tensor(lost[i], dtype=torch.int64))
+            x = torch.einsum("thd,jhd->htj", q[rows].double(), k) * d ** -0.5
+            p = torch.where(seen.any(-1)[None, :, None], torch.softmax(x.masked_fill(~seen, -torch.inf), -1), 0.0)
+            big = (torch.einsum("thd,jhd->htj", q[rows].double().abs(), k.abs()) * d ** -0.5).masked_fill(~seen, 0).amax(-1).T
+            top = torch.where(seen[None], v.abs().amax(-1).T[:, None, :], 0).amax(-1).T
+            want = torch.einsum("htj,jhd->thd", p, v)
+            assert ((got[rows] - want).abs() <= tolerance(want, top, big, dtype, n, d)).all(), (counts, i)
+        with pytest.raises(llaisys.LlaisysError) as e:
+            f.cache.check()
+        assert e.value.status == Status.KERNEL
+    # a sequence that does not exist and holds nothing: nothing is looked up
+    for starts in (None, i32([0, 1]), i32([0, 1000])):
+        out = torch.full((1000, nh, d), 9.0, dtype=TORCH[dtype], device="cuda")
+        n = 1 if starts is None else int(starts[1])
+        f.cache.attention_dev(0, out, torch.ones_like(out), i32([77]), starts, i32([0]), n_seqs=1, total_q=n, max_q_len=n, max_kv_len=max(lens), nh=nh,
+                              scale=1.0, stream=stream(), window=window)
+        assert (out[:n] == 0).all() and (out[n:] == 9).all()
+        f.cache.check()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype,nh,nkvh,d", [("bf16", 2, 2, 128), ("f16", 4, 1, 64), ("f32", 12, 2, 96), ("bf16", 16, 1, 256)])
 def test_tables_that_are_full(cuda_device, dtype, nh, nkvh, d):
     """Sequences that end in the last block of their tables: nothing behind it is looked up."""
