@@ -618,7 +618,7 @@ __global__ void __launch_bounds__(Shape<D, R>::kThreads, Shape<D, R>::kCtas) att
             for (int o = S::kRowThreads / 2; o > 0; o >>= 1) {
                 most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
             }
-            const int e = max(-100, min(126, (__float_as_int(most) >> 23) - 127));
+            const int e = max(-100, min(127, (__float_as_int(most) >> 23) - 127));
             const float up = power_of_two(14 - e);
             float sum = 0.f;
 #pragma unroll
@@ -648,7 +648,7 @@ __global__ void __launch_bounds__(Shape<D, R>::kThreads, Shape<D, R>::kCtas) att
             }
             if (my_part == 0) {
                 s_factor[my_row] = factor;
-                s_lack[my_row] = 128.f * sum * factor;
+                s_lack[my_row] = 128.f * sum; // (times the factor it need not be a number where the scores are)
                 s_pos[my_row] = min(my_packed, f.row0 + f.rows - 1) / p.group + f.off;
             }
         }
@@ -800,7 +800,7 @@ __global__ void __launch_bounds__(Shape<D, R>::kThreads, Shape<D, R>::kCtas) att
                 const float2 scales = *reinterpret_cast<const float2 *>(my_ring + slot[b] * S::kTile + quant_scales_at(d));
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const float by = factor[h] * scales.x * (kBiased ? 0x1p24f : 1.f), less = kBiased ? -lack[h] * scales.x : 0.f;
+                    const float unit = factor[h] * scales.x, by = unit * (kBiased ? 0x1p24f : 1.f), less = kBiased ? -lack[h] * unit : 0.f;
 #pragma unroll
                     for (int k = 0; k < kOfRow; ++k) {
                         float &x = R == 16 ? s[b][k >> 1][2 * h + (k & 1)] : s[b][0][2 * k + h];

@@ -702,7 +702,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_quant_tc_kernel(QuantCh
                 for (int o = kRowLanes / 2; o > 0; o >>= 1) {
                     most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
                 }
-                const int e = max(-100, min(126, (__float_as_int(most) >> 23) - 127));
+                const int e = max(-100, min(127, (__float_as_int(most) >> 23) - 127));
                 const float up = power_of_two(14 - e);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {

@@ -604,6 +604,26 @@ def test_long_chunks_behind_values_that_are_zero_for_long(cuda_device, store):
     cache.check()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("store", ["i8", "f8"])
+@pytest.mark.parametrize("dtype,nh", [("bf16", 4), ("f32", 4), ("bf16", 16)])
+def test_queries_at_the_end_of_their_range(cuda_device, dtype, store, nh):
+    """Keys that are zero have score 0 whatever the queries: the mean of the values."""
+    n, d = 400, 64
+    cache = constant_rows(1, n, 1, d, dtype, store, lambda t: 0.0 * t, lambda t: 1.0 + t // 16 % 2)
+    q = torch.full((n, nh, d), torch.finfo(TORCH[dtype]).max, dtype=TORCH[dtype], device="cuda")
+    q[::3] = -2.0 ** 121
+    out = torch.empty_like(q)
+    tol = torch.finfo(TORCH[dtype]).eps / 2 + (2.0 ** -20 if dtype == "f32" else 2.0 ** -11 * 1.01)
+    for rows in (1, 3, n):
+        starts = None if rows == 1 else i32([0, rows])
+        cache.attention_dev(0, out, q, i32([0]), starts, i32([n]), n_seqs=1, total_q=rows, max_q_len=rows, max_kv_len=n, nh=nh, scale=1.0,
+                            stream=stream())
+        value = (1.0 + torch.arange(n).double() // 16 % 2).cumsum(0) / torch.arange(1, n + 1)
+        assert ((out[:rows].cpu().double() - value[n - rows:, None, None]).abs() <= 2 * tol).all(), rows
+    cache.check()
+
+
 # ---- a step, planned and run ----------------------------------------------------------------------------------------------
 
 
