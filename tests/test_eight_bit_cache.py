@@ -627,25 +627,28 @@ def test_queries_at_the_end_of_their_range(cuda_device, dtype, store, nh):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype,nh,d", [("f16", 4, 64), ("bf16", 4, 128), ("f16", 16, 64), ("bf16", 2, 256)])
 def test_long_sums_of_integers_do_not_drift(cuda_device, dtype, nh, d):
-    """Means of 60000 integers, 15000 of them to a warp. Weights are powers of two and codes are what was appended, so that nothing is rounded but sums, by
-    2^-23 of the sum an addition of 16 tokens: in 256 tokens, 16 additions to at most 255 w a token and 16 to w a token that count 128 times; and n / 16
-    additions to what was there, which after t tokens of either sign (59 rms) is not over 4 * 59 sqrt(t) w: 236 / 16 * 2 / 3 sqrt(n) of them a token. A few
-    more where parts join, of the mean itself, which is below one."""
+    """Means of 60000 values, 15000 of them to a warp, all of one scale s and of weight w = f16(s). Besides w, which is off by 2^-11 of itself, only sums
+    are rounded, by 2^-23 of the sum an addition of 16 tokens: in 256 tokens, 16 additions to at most 255 w a token and 16 to w a token that count 128
+    times; and n / 16 additions to what was there, which after t codes of either sign (59 rms) is not over 4 * 59 sqrt(t) w: 236 / 16 * 2 / 3 sqrt(n) of
+    them a token. A few more where parts join, of the mean itself, which is below one code."""
     n, seqs = 60000, 3 * torch.cuda.get_device_properties(0).multi_processor_count
     pages = n // 16
     cache = llaisys.PagedKVCache.quantized(pages, 1, d, dtype=NAMES[dtype], max_seqs=1, max_pages_per_seq=pages)
-    v = torch.randint(-100, 101, (n, 1, d), generator=torch.Generator().manual_seed(3))
-    v[::32, 0, 0], v[16::32, 0, 0] = 127, -127  # a scale of one
+    v = (torch.randint(-100, 101, (n, 1, d), generator=torch.Generator().manual_seed(3)) * 1.4719).to(TORCH[dtype])
+    v[::32, 0, 0], v[16::32, 0, 0] = 187, -187  # the largest of every block
+    values = Definition(1, d, "i8")
+    values.append(0, v.float().numpy())
+    unit = 187 / 127
     cache.reserve(cache.add_seq(), n)
     cache.flush()
-    cache.append_dev(0, torch.zeros(n, 1, d, dtype=TORCH[dtype], device="cuda"), v.to(TORCH[dtype]).cuda(), i32([0] * n), i32(range(n)), n, stream())
+    cache.append_dev(0, torch.zeros(n, 1, d, dtype=TORCH[dtype], device="cuda"), v.cuda(), i32([0] * n), i32(range(n)), n, stream())
     q = torch.randn(seqs, nh, d, generator=torch.Generator().manual_seed(4)).to(TORCH[dtype]).cuda()
     part = torch.empty(seqs, nh, d + 2, device="cuda")
     cache.decode_partial_dev(0, part, q, i32([0] * seqs), i32([n] * seqs), seqs, n, nh, 0.1, stream())
-    want = v[:, 0].double().mean(0)
-    off = (part[..., :d].cpu().double() - want).abs()
-    assert want.abs().max() < 1
-    assert off.max() <= (16 * (255 + 128) + 236 / 24 * 15000 ** 0.5 + 64) * 2.0 ** -23
+    want = torch.from_numpy(values.worth()).double()[:, 0].mean(0)
+    off = (part[..., :d].cpu().double() - want).abs() - want.abs() * 2.0 ** -11
+    assert want.abs().max() < unit
+    assert off.max() <= (16 * (255 + 128) + 236 / 24 * 15000 ** 0.5 + 64) * 2.0 ** -23 * unit, off.max() / unit * 2.0 ** 23
     cache.check()
 
 
