@@ -291,6 +291,42 @@ def test_append_of_many_rows_among_them_some_without_a_place(cuda_device, dtype,
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("store", ["i8", "f8"])
+@pytest.mark.parametrize("dtype,nkvh,d,page", [("bf16", 2, 128, 16), ("f16", 8, 32, 48), ("f32", 4, 64, 32), ("f32", 1, 256, 16)])
+def test_many_rows_in_a_call(cuda_device, dtype, store, nkvh, d, page):
+    """Several thousand rows at a time, appended from inside blocks on and read back in one call: in order, out of order, and with rows in between that
+    do not exist. Every number equals the definition's."""
+    rng = np.random.default_rng(d)
+    few = 64 * torch.cuda.get_device_properties(0).multi_processor_count // (2 * nkvh)  # rows up to which a warp takes one
+    lens = [int(x) for x in rng.integers(0, 40, 150)] + [few, 300]
+    f = Filled(lens, nkvh, d, dtype, store, page, extra=2 * few)
+    new = [int(x) for x in rng.integers(0, 50, 150)] + [few + 13, 7]
+    f.append([(i, n, m) for i, (n, m) in enumerate(zip(lens, new)) if m])
+    f.append([(i, n + m, 1) for i, (n, m) in enumerate(zip(lens, new))])
+    seq = np.concatenate([[s] * (n + m + 1) for s, n, m in zip(f.seqs, lens, new)])
+    pos = np.concatenate([np.arange(n + m + 1) for n, m in zip(lens, new)])
+    assert len(seq) > few
+    wants = [torch.from_numpy(np.concatenate([x.worth() for x in side])).to(TORCH[dtype]) for side in (f.k, f.v)]
+    mixed = rng.permutation(len(seq))
+    gaps = np.sort(rng.choice(len(seq), 200, replace=False))
+    for order, bad in ((np.arange(len(seq)), False), (mixed, False), (np.arange(len(seq)), True)):
+        s, p = seq[order].copy(), pos[order].copy()
+        if bad:
+            s[gaps[:100]], p[gaps[100:]] = 99999, np.where(gaps[100:] % 2, -1, 1 << 22)
+        got = [torch.full((len(seq), nkvh, d), 7.0, dtype=TORCH[dtype], device="cuda") for _ in range(2)]
+        f.cache.gather_dev(0, *got, i32(s), i32(p), len(seq), stream())
+        for g, want in zip(got, wants):
+            want = want[torch.from_numpy(order)]
+            if bad:
+                want[torch.from_numpy(gaps)] = 7.0
+            assert torch.equal(g.cpu(), want)
+        if bad:
+            with pytest.raises(llaisys.LlaisysError):
+                f.cache.check()
+    f.cache.check()
+
+
+@pytest.mark.gpu
 def test_host_forms_fork_and_prefix(cuda_device):
     f = Filled([37, 5], 2, 64, "f16", "i8", 16, extra=20)
     k, v = f.rows(4), f.rows(4)
