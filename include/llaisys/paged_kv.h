@@ -163,7 +163,8 @@ LLAISYS_API int llaisysPagedKVFlush(llaisysPagedKV_t kv);
  * before waiting, and touches q, K/V, workspace and outputs only after the kernel directly before it has completed. */
 LLAISYS_API int llaisysPagedKVSetLaunchOverlap(llaisysPagedKV_t kv, int enable);
 /* Polls after which a wait of one part of the chunk attention kernel for another gives up (default 1 << 20, about a second at worst; another
- * limit is for tests and taken by the bf16 form without window, factor or penalty). A call in which one ran out leaves its
+ * limit is for tests and taken by the bf16 form without window, factor or penalty; of a cache held in 8 bits by the kernel of short calls and, for
+ * heads of 128, integers and no window, by that of chunks). A call in which one ran out leaves its
  * output undefined and is reported by llaisysPagedKVCheck; nothing of it is left running. */
 LLAISYS_API int llaisysPagedKVSetWaitLimit(llaisysPagedKV_t kv, uint32_t polls);
 /* LLAISYS_KERNEL_* of this cache's most recent attention call (-1 for a null handle). */

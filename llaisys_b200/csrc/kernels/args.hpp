@@ -64,6 +64,7 @@ struct QuantView {
     int32_t table_rows = 0, table_stride = 0;
     bool f8 = false; // codes are e4m3 numbers, not integers
     bool overlap_launch = false; // as in KVView
+    uint32_t wait_limit = 1u << 20;
 };
 
 // The arrays of a step from its requests' lengths (see llaisysPagedPlanDev).

@@ -38,7 +38,7 @@ constexpr int kRows = 16;
 constexpr int kMinPiece = 12; // units of the shortest piece
 constexpr int kTileUnits = 24; // what a row tile costs besides its blocks, in units of a block's time
 constexpr int kSnap = 8;       // a piece's border that comes this near a row tile's first or last block moves there: no fragments of a few blocks
-constexpr uint32_t kWaitLimit = 1u << 20;
+constexpr uint32_t kDrainLimit = 1u << 20;
 constexpr int kErrTimeout = 8;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kShift = 14.f; // weights are 2^14 times what they stand for
@@ -702,13 +702,13 @@ __global__ void __launch_bounds__(Shape<D, R>::kThreads, Shape<D, R>::kCtas) att
             for (int b = 0; b < kPair; ++b) {
                 live[b] = i + b < blocks;
                 slot[b] = (taken + (live[b] ? b : 0)) % S::kSlots;
-                dead = dead || !mbar_wait_bounded(bars + 8 * slot[b], ((taken + (live[b] ? b : 0)) / S::kSlots) & 1, kWaitLimit);
+                dead = dead || !mbar_wait_bounded(bars + 8 * slot[b], ((taken + (live[b] ? b : 0)) / S::kSlots) & 1, p.kv.wait_limit);
             }
             if (__any_sync(0xffffffffu, dead)) {
                 dead = true;
                 // what else is on its way lands before the CTA ends
                 for (uint32_t c = taken; c != asked; ++c) {
-                    mbar_wait_bounded(bars + 8 * (c % S::kSlots), (c / S::kSlots) & 1, 1u << 12);
+                    mbar_wait_bounded(bars + 8 * (c % S::kSlots), (c / S::kSlots) & 1, kDrainLimit);
                 }
                 if (lane == 0) {
                     atomicOr(p.error_flag, kErrTimeout);

@@ -120,7 +120,7 @@ __device__ __forceinline__ uint32_t pack_out(float a, float b, bool bf16) {
 }
 __device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }
 
-template <int D, bool kF8, bool kWin>
+template <int D, bool kF8, bool kWin, bool kShortWaits = false>
 __global__ void __launch_bounds__(kThreads, 1) attention_quant_tc_kernel(QuantChunkParams p) {
     using S = Shape<D>;
     constexpr int kStages = S::kStages, kStageBytes = S::kStageBytes, kQBytes = S::kQBytes, kQPiece = S::kQPiece, kKPiece = S::kKPiece,
@@ -298,7 +298,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_quant_tc_kernel(QuantCh
     auto bar = [&](int which) { return bars_u32 + uint32_t(which) * 8; };
     // False when the wait ran out here or somewhere else in the CTA (lanes may disagree on that); raises the flag that ends the others.
     auto wait = [&](int which, uint32_t parity) {
-        const bool ok = wait_or_abort(bar(which), parity & 1u, s_abort);
+        const bool ok = wait_or_abort(bar(which), parity & 1u, s_abort, kShortWaits ? p.kv.wait_limit : kMbarWaitLimit);
         if (!ok) {
             *s_abort = 1;
         }
@@ -431,8 +431,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_quant_tc_kernel(QuantCh
             auto step = [&]() { // to the next block: its tiles
                 const int at = heard % kFeedSlots;
                 ok = __all_sync(0xffffffffu, wait(kBarFound + at, heard / kFeedSlots)) && ok;
-                tiles[0] = s_feed[at * kPagesPerBlock + block_a].place;
-                tiles[1] = s_feed[at * kPagesPerBlock + block_a + 2].place;
+                tiles[0] = ok ? s_feed[at * kPagesPerBlock + block_a].place : kNone; // (where the wait ran out nobody may have written there yet)
+                tiles[1] = ok ? s_feed[at * kPagesPerBlock + block_a + 2].place : kNone;
                 more = ok && tiles[0] != kEnd;
             };
             constexpr int kHalfVecs = kVecs / 2; // 16-byte loads of a unit of V from either tile
@@ -1078,7 +1078,9 @@ bool attention_quant_tc(stream_t stream, llaisysDataType_t dtype, const QuantVie
     };
     auto launch = [&](auto d) {
         constexpr int D = decltype(d)::value;
-        if (batch.window > 0) {
+        if (D == 128 && kv.wait_limit != kMbarWaitLimit && !kv.f8 && batch.window == 0) { // (a limit that tests set)
+            start(attention_quant_tc_kernel<128, false, false, true>, Shape<128>::kBytes);
+        } else if (batch.window > 0) {
             start(kv.f8 ? attention_quant_tc_kernel<D, true, true> : attention_quant_tc_kernel<D, false, true>, Shape<D>::kBytes);
         } else {
             start(kv.f8 ? attention_quant_tc_kernel<D, true, false> : attention_quant_tc_kernel<D, false, false>, Shape<D>::kBytes);

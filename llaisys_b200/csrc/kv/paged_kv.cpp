@@ -543,6 +543,7 @@ kernels::QuantView PagedKV::quantView(size_t layer) const {
     v.table_stride = int32_t(_cfg.max_pages_per_seq);
     v.f8 = _cfg.store == LLAISYS_DTYPE_F8;
     v.overlap_launch = _overlap;
+    v.wait_limit = _wait_limit;
     return v;
 }
 

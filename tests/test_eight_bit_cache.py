@@ -1011,6 +1011,40 @@ def test_two_caches_on_two_streams_and_graphs(cuda_device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("form", ["decode", "pieces", "chunks"])
+def test_waits_that_run_out_are_reported(cuda_device, form):
+    """With a limit of a few polls the waits inside a healthy pipeline run out, from the first on or somewhere in the middle: the call ends, is reported,
+    and the next one, with the limit as it was, gives the bits of the one before."""
+    f = Filled([1700, 1, 45, 4300, 333], 2, 128, "bf16", "i8")
+    counts = dict(decode=[1] * 5, pieces=[3, 1, 5, 2, 4], chunks=[700, 1, 40, 300, 333])[form]
+    total = sum(counts)
+    q = torch.randn(total, 12, 128, generator=torch.Generator().manual_seed(5)).bfloat16().cuda()
+    ids, starts, lens = i32(f.seqs), i32([0, *np.cumsum(counts).tolist()]), i32([1700, 1, 45, 4300, 333])
+    out = torch.empty_like(q)
+
+    def attend():
+        out.fill_(torch.nan)
+        f.cache.attention_dev(0, out, q, ids, None if form == "decode" else starts, lens, n_seqs=5, total_q=total, max_q_len=max(counts), max_kv_len=4300,
+                              nh=12, scale=0.1, stream=stream())
+        torch.cuda.synchronize()
+        f.cache.check()
+        return out.clone()
+
+    first = attend()
+    assert torch.isfinite(first).all()
+    assert f.cache.last_kernel() == (llaisys.Kernel.EIGHT_BIT_TC if form == "chunks" else llaisys.Kernel.EIGHT_BIT)
+    for polls in (0, 1, 2, 4, 8, 16, 64, 0):
+        f.cache.set_wait_limit(polls)
+        try:
+            attend()
+            assert polls > 0
+        except llaisys.LlaisysError as e:
+            assert e.status == Status.KERNEL
+        f.cache.set_wait_limit(1 << 20)
+        assert torch.equal(attend(), first), polls
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("held,rows", [(2000, 900), (40, 40)])
 def test_queries_end_with_the_call(cuda_device, held, rows):
     """q_starts that go on behind total_q: the queries there are none of the call's."""
