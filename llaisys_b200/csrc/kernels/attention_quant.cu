@@ -248,7 +248,7 @@ __device__ __forceinline__ uint4 lds128(uint32_t addr) {
 // The blocks of a fragment that are a warp's: the warps take kPair neighbours each, in turn. Lanes hold the tiles' places, 32 blocks at a time
 // and the next 32 ahead.
 struct Feed {
-    const int32_t *table; // null: no such sequence
+    int row; // of the table; -1: no such sequence
     int count, first, kept, gap, kvh;
     int now, next;
 };
@@ -275,13 +275,10 @@ __device__ __forceinline__ int tile_place(const QuantParams &p, const Feed &f, i
     int block = f.first + S::kWarps * (k - k % S::kPair) + k % S::kPair;
     block = block < f.kept ? block : block + f.gap;
     const int entry = p.kv.blocks_per_page == 1 ? block : block / p.kv.blocks_per_page;
-    if (f.table == nullptr || entry >= p.kv.table_stride) {
-        atomicOr(p.error_flag, f.table == nullptr ? kErrBadSeq : kErrBadPosition);
-        return -1;
-    }
-    const int page = f.table[entry];
-    if (page < 0 || page >= p.kv.num_pages) {
-        atomicOr(p.error_flag, kErrBadPage);
+    const int page = p.kv.block_table[int64_t(max(f.row, 0)) * p.kv.table_stride + min(entry, p.kv.table_stride - 1)]; // (in the table whatever comes of it)
+    const int what = f.row < 0 ? kErrBadSeq : entry >= p.kv.table_stride ? kErrBadPosition : page < 0 || page >= p.kv.num_pages ? kErrBadPage : 0;
+    if (what != 0) {
+        atomicOr(p.error_flag, what);
         return -1;
     }
     return (page * p.kv.blocks_per_page + block - entry * p.kv.blocks_per_page) * p.kv.nkvh + f.kvh;
@@ -291,7 +288,7 @@ template <typename S>
 __device__ __forceinline__ Feed open_feed(const QuantParams &p, const Fragment &f, int seq, int first, int lane) {
     Feed feed;
     const int blocks = f.b1 - f.b0 - first, sweep = S::kPair * S::kWarps;
-    feed.table = seq >= 0 && seq < p.kv.table_rows ? p.kv.block_table + int64_t(seq) * p.kv.table_stride : nullptr;
+    feed.row = seq >= 0 && seq < p.kv.table_rows ? seq : -1;
     feed.first = f.b0 + first;
     feed.count = blocks <= 0 ? 0 : blocks / sweep * S::kPair + min(blocks % sweep, S::kPair);
     feed.kept = f.kept;
@@ -429,7 +426,7 @@ __global__ void __launch_bounds__(Shape<D, R>::kThreads, Shape<D, R>::kCtas) att
         int64_t *sums = reinterpret_cast<int64_t *>(s_merge);
         const int per = (p.n_seqs + kThreads - 1) / kThreads, a0 = min(tid * per, p.n_seqs), a1 = min(a0 + per, p.n_seqs);
         int64_t mine = 0;
-        const int seq0 = a0 < a1 ? p.seq_ids[a0] : -1; // (on its way with the lengths)
+        const int seq0 = p.seq_ids[min(a0, p.n_seqs - 1)]; // (on its way with the lengths)
         for (int a = a0; a < a1; ++a) {
             const SeqGeom g = seq_geom(p, a);
             mine += units_before(p, g, g.tiles) * p.kv.nkvh;

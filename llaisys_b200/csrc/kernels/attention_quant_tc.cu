@@ -381,21 +381,17 @@ __global__ void __launch_bounds__(kThreads, 1) attention_quant_tc_kernel(QuantCh
                 }
                 const int32_t *table = p.kv.block_table + (long long)(known ? seq : 0) * p.kv.table_stride;
                 auto find = [&](int blk0) {
-                    Found found{kNone, 0.f, 0.f};
                     const int b = blk0 + lane / kPagesPerBlock;
                     const int at = min((kWin && b >= w.g.kept_blocks ? b + f.gap : b) * kPagesPerBlock + lane % kPagesPerBlock, last);
-                    if (at >= 0 && known) { // (else: no token at all, no sequence)
-                        const int entry = p.kv.blocks_per_page == 1 ? at : at / p.kv.blocks_per_page, page = table[entry];
-                        if (page < 0 || page >= p.kv.num_pages) {
-                            atomicOr(p.error_flag, kErrBadPage);
-                        } else {
-                            found.place = (page * p.kv.blocks_per_page + at - entry * p.kv.blocks_per_page) * p.kv.nkvh + f.kvh;
-                            const float2 scales = __ldcg(reinterpret_cast<const float2 *>(p.kv.base + (long long)found.place * p.kv.tile_bytes + quant_scales_at(D)));
-                            found.s_k = scales.x;
-                            found.s_v = scales.y;
-                        }
+                    // (what is loaded lies in the table and in the pool whatever comes of it: where there is no token, no sequence or no page, page 0's)
+                    const int in_table = max(at, 0), entry = p.kv.blocks_per_page == 1 ? in_table : in_table / p.kv.blocks_per_page, page = table[entry];
+                    const bool named = at >= 0 && known, there = named && page >= 0 && page < p.kv.num_pages;
+                    const int place = ((there ? page : 0) * p.kv.blocks_per_page + in_table - entry * p.kv.blocks_per_page) * p.kv.nkvh + f.kvh;
+                    const float2 scales = __ldcg(reinterpret_cast<const float2 *>(p.kv.base + (long long)place * p.kv.tile_bytes + quant_scales_at(D)));
+                    if (named && !there) {
+                        atomicOr(p.error_flag, kErrBadPage);
                     }
-                    return found;
+                    return there ? Found{place, scales.x, scales.y} : Found{kNone, 0.f, 0.f};
                 };
                 Found group = find(f.b0), next_group = find(f.b0 + kGroup);
                 for (int i = 0; i < n && alive; ++i) {
@@ -437,22 +433,21 @@ __global__ void __launch_bounds__(kThreads, 1) attention_quant_tc_kernel(QuantCh
             };
             constexpr int kHalfVecs = kVecs / 2; // 16-byte loads of a unit of V from either tile
             uint4 raw[2 * kHalfVecs];
-            const uint4 none = kF8 ? make_uint4(0, 0, 0, 0) : make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
-            // Where the next unit's words come from: the low half of `raw` from one place on, the high half from another (null: no tile).
-            const uint4 *from[2] = {nullptr, nullptr};
-            auto tile_of = [&](int b) { return tiles[b] >= 0 ? reinterpret_cast<const uint4 *>(p.kv.base + (long long)tiles[b] * tile_bytes) + lane : nullptr; };
+            // Where the next unit's words come from: the low half of `raw` from one place on, the high half from another. Where there is no tile the pool's
+            // first one stands in: codes are numbers, and whoever they are multiplied with has the weight 0 (and, behind the last block, nobody asks).
+            const uint4 *from[2];
+            auto tile_of = [&](int b) { return reinterpret_cast<const uint4 *>(p.kv.base + (long long)max(tiles[b], 0) * tile_bytes) + lane; };
             auto point_k = [&](int b) {
                 from[0] = tile_of(b);
-                from[1] = from[0] != nullptr ? from[0] + 32 * kHalfVecs : nullptr;
+                from[1] = from[0] + 32 * kHalfVecs;
             };
             auto point_v = [&](int half) {
 #pragma unroll
                 for (int b = 0; b < 2; ++b) {
-                    from[b] = tile_of(b);
-                    from[b] = from[b] != nullptr ? from[b] + kQuantTokens * D / 16 + 32 * kHalfVecs * half : nullptr;
+                    from[b] = tile_of(b) + kQuantTokens * D / 16 + 32 * kHalfVecs * half;
                 }
             };
-            auto fetch = [&](int k) { raw[k] = from[k / kHalfVecs] != nullptr ? __ldcg(from[k / kHalfVecs] + 32 * (k % kHalfVecs)) : none; };
+            auto fetch = [&](int k) { raw[k] = __ldcg(from[k / kHalfVecs] + 32 * (k % kHalfVecs)); };
             int stage = 0;
             uint32_t turn = 0;
             auto take_stage = [&]() {
@@ -531,12 +526,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_quant_tc_kernel(QuantCh
                     if (half == 0) {
                         point_v(1);
                     } else {
-                        step(); // (V is asked for; K of the next block comes next, or nothing)
-                        if (more) {
-                            point_k(0);
-                        } else {
-                            from[0] = from[1] = nullptr;
-                        }
+                        step(); // (V is asked for; K of the next block comes next)
+                        point_k(0);
                     }
 #pragma unroll
                     for (int v = 0; v < kHalfVecs; ++v) {
@@ -680,11 +671,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_quant_tc_kernel(QuantCh
 #pragma unroll
             for (int it = 0; it < kIter; ++it) {
                 const int r = row / kRowLanes + it * kAtOnce, cc = row % kRowLanes, x = f.qb * kRows + h * kHalf + r, t = per_group(x);
-                vals[it] = make_uint4(0u, 0u, 0u, 0u);
-                if (t < g.q_len) {
-                    vals[it] = *reinterpret_cast<const uint4 *>(static_cast<const char *>(p.q) + cc * 16 +
-                                                                ((long long)(g.q_start + t) * p.nh + f.kvh * p.group + (x - t * p.group)) * (D * 2));
-                }
+                const uint4 had = *reinterpret_cast<const uint4 *>(static_cast<const char *>(p.q) + cc * 16 + // (rows past the chunk: its last one)
+                                                                   ((long long)(g.q_start + min(t, g.q_len - 1)) * p.nh + f.kvh * p.group + (x - t * p.group)) * (D * 2));
+                vals[it] = t < g.q_len ? had : make_uint4(0u, 0u, 0u, 0u);
             }
 #pragma unroll
             for (int it = 0; it < kIter; ++it) {
