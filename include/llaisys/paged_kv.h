@@ -88,9 +88,10 @@ LLAISYS_API int llaisysPagedKVDestroy(llaisysPagedKV_t kv);
  * a call appends to a block (all in f32, products and quotients rounded once):
  *     s' = max(s, max|x| / M, 2^-100)   over the rows' numbers x; s only where the first of them does not go to the block's slot 0
  *     c  = round(x * (1 / s'))          to nearest, ties to even;   tokens in front of the rows, where s' > s:  c = round(c * (s * (1 / s')))
- * so that a block filled token by token is rounded again only when its scale grows. A block that a NaN or an infinity is appended to
- * gets the scale NaN, and attention of every query that reads the block is NaN, until its slot 0 is written again. Tokens that
- * were never written have no value.
+ * so that a block filled token by token is rounded again only when its scale grows. Tokens of the block behind the rows keep their codes,
+ * whatever becomes of the scale: a call that writes tokens again leaves those behind them in the block without a value (the other caches
+ * leave them as they were), and so are tokens that were never written. A block that a NaN or an infinity is appended to gets the scale NaN,
+ * and attention of every query that sees a token of the block is NaN, until its slot 0 is written again.
  * The block manager, llaisysPagedKVAppend(Dev), Gather(Dev), llaisysPagedAttentionDecode(Dev), ...Prefill(Dev), ...DecodePartial(Dev) and
  * llaisysPagedAttentionOptDev (mixers.h) take such a cache with rows, queries and outputs of `dtype`; every other call returns
  * LLAISYS_E_UNSUPPORTED. The rows that one append call brings to a block must be neighbours in the call, in the order of their
@@ -271,8 +272,10 @@ LLAISYS_API int llaisysPagedAttentionPrefillDev(llaisysPagedKV_t kv, size_t laye
  *   block_table_dev [table_rows][table_stride]: entries [pages(held), pages(held + new)) of request i, requests in order, take
  *                                 free_pages_dev[0], [1], ...; NULL free_pages_dev: the table is complete already and only read
  *   status_dev [2]                pages taken, and LLAISYS_PLAN_ bits
- * Any output may be NULL, and so may the table when neither slots nor growth are wanted; no output lies over an input. Rows behind the last request's, up to n_rows, are -1
- * (such rows are skipped by appends to a cache held in 8 bits). A request may appear once.
+ * Any output may be NULL, and so may the table when neither slots nor growth are wanted; no output lies over an input or over another one. Rows
+ * behind the last request's, up to n_rows, are -1: appends to a cache held in 8 bits skip such rows, those to other caches flag them and store the
+ * others. A request may appear once. Growth is for callers that keep pages and table themselves: a cache's block manager knows nothing of pages
+ * that a plan takes, and gives pages and entries of its own.
  * What cannot be done is left out and flagged, never written elsewhere: rows behind n_rows count as not brought, in every array (the requests they
  * belong to may bring them in a later step); too few free pages take none at all; negative counts and sums over 2^31 - 1 count as nothing brought; a
  * request whose row or last page lies outside the table gets no page. Rows that have no page for these reasons are -1 in all three arrays, so that

@@ -6,14 +6,15 @@
 // so that the f16 weights w f lie below 2^15 however far the scales are apart, and the smallest normal one is 2^-28 of the largest. Queries are
 // scaled by a power of two to below 2^15, row by row. For 32-bit activations q and the weights are taken as two f16 numbers each (22 bits), and
 // the tensor cores, which cut their sums where additions round, add up only 16 dims or 32 tokens at a time: over 8000 tokens of
-// 256 dims the error is 5.7e-7 of the outputs instead of 1.2e-6, for 0.5 us of 29.6 (24 sequences, windows of 2000 tokens).
+// 256 dims the error is 5.7e-7 of the outputs instead of 1.2e-6, for 0.5 us of 29.6 (24 sequences, windows of 2000 tokens). The sum of the weights
+// loses tokens whose x + e lies 140 below M: of blocks whose V scales are that many powers of two below the largest, at like scores.
 //
 // Bound: the pool's bytes. 16 tokens of a kv head are a tile of 32 d + 16 bytes that lies in one piece, so one bulk copy fetches it.
 //
 // Work. A row is (query, head of the group); 16 packed rows of a sequence and kv head are a TILE of rows, which visits its visible blocks of 16
-// tokens, one UNIT each, and one more unit for what a tile costs besides. All units, in the order (sequence, row tile, kv head, block), form a line
+// tokens, one UNIT each, and kTileUnits more for what a tile costs besides. All units, in the order (sequence, row tile, kv head, block), form a line
 // that is cut into equal pieces, one per CTA. A piece covers the end of one row tile, whole ones and the beginning of another; each such
-// FRAGMENT is worked on by all eight warps, every one with every eighth block, and merged in shared memory. A fragment that is its whole
+// FRAGMENT is worked on by all warps, which take its blocks in turn (heads of up to 128: two at a time), and merged in shared memory. A fragment that is its whole
 // row tile stores its rows; otherwise it leaves sums and maxima in a slot of the workspace, and the one that arrives last merges them, in the
 // order of the CTAs. Nobody waits for another CTA.
 // A warp feeds itself: it has a ring of slots of its own, asks for a block as soon as it has read the one that lay in the slot, and looks one

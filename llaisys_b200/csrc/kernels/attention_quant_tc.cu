@@ -14,9 +14,9 @@
 // [dim][keys], both K-major in the 128-byte swizzle. Lanes whose rows would meet in the same banks take their words in another order: K's odd tokens
 // 16 dims apart from the even ones, V's odd dims from the second of two blocks that lie 32 keys apart.
 //
-// Measured, 12 / 2 heads of 128: eight chunks of 512 tokens behind up to 8192, integers, 143 us (800 TFLOP/s); a prompt of 5000, 32 / 8 heads, e4m3, 284 us
-// (720); 16-bit pages take the other kernel 113 and 199. With operands that nobody widens (a probe) it is 141 and 275: what bounds a block is the
-// chain scores -> scale -> maximum -> exponentials -> products of a half.
+// Measured, 12 / 2 heads of 128: eight chunks of 512 tokens behind up to 8192, integers, 149 us (776 TFLOP/s); a prompt of 5000, 32 / 8 heads,
+// e4m3, 280 us (730); 16-bit pages take the other kernel 113 and 199. With operands that nobody widens (a probe) it is 2 and 9 us less: what bounds a block
+// is the chain scores -> scale -> maximum -> exponentials -> products of a half. (Loads of codes under a condition, for tiles that may not exist: 155 us.)
 //
 // Roles: warps 0-3 and 4-7 softmax of the halves, 8 and 9 MMA issue, 10-13 the operands: two blocks of 16 keys each, of K, then of V, of every block of
 // 128. Waits are bounded as in the other kernel; nothing asynchronous is left behind but MMAs, which the issuers see through.

@@ -61,11 +61,12 @@ __device__ __forceinline__ int tile_gap(const SeqGeom &g, int qb) {
 }
 __device__ __forceinline__ int tile_blocks(const SeqGeom &g, int qb) { return (tile_kv_hi(g, qb) + kKeys - 1) / kKeys - tile_gap(g, qb); }
 
-// sum of floor((2 i + b) / m) over i < n, for 0 <= b and m <= 8
+// sum of floor((2 i + b) / m) over i < n, for 0 <= b and m <= 32. Callers see to it that the sum fits 32 bits; n (n - 1) may not where a / m is 0, and
+// counts for nothing there.
 __device__ __forceinline__ int floor_sum(int n, int m, int b) {
     int sum = 0, a = 2;
     while (n > 0) {
-        sum += n * (n - 1) / 2 * (a / m) + n * (b / m);
+        sum += (a >= m ? n * (n - 1) / 2 * (a / m) : 0) + n * (b / m);
         a %= m;
         b %= m;
         const int y = a * n + b;

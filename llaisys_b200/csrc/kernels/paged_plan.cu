@@ -5,8 +5,9 @@
 // requests by itself -- a CHUNK of neighbours per thread, a sum over warps and CTA -- and then writes its share of the rows, four at a time
 // per thread, and of the requests. A row finds its chunk by bisection of the chunks' sums in shared memory and its request by walking the
 // chunk. (Handing the sums from CTA to CTA would read the lengths once instead of once per CTA; they are 8 bytes a request out of L2.)
-// 64 requests of one token: 5.8 us on the device; 4000 prompts of 1 to 512 tokens (a million rows, 16 MB): 15.5 us, a third of it the sums that every
-// CTA makes. (One CTA that went through the requests one by one: 30.8 and 2530 us.)
+// 64 requests of one token: 6.2 us on the device; 4000 prompts of 1 to 512 tokens (a million rows, 16 MB): 17.2 us, a third of it the sums that every
+// CTA makes. (One CTA that went through the requests one by one: 30.8 and 2530 us. Plans that looked for neither rows to drop nor rows without a page
+// took 5.8 and 15.7.)
 #include "kernels.hpp"
 #include "launch_utils.cuh"
 
