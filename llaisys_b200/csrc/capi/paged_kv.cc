@@ -157,6 +157,13 @@ int llaisysPagedPlanDev(llaisysDeviceType_t device_type, int device_id, const Ll
                 throw StatusError(LLAISYS_E_INVALID, "paged plan: an array is not aligned to its elements, or an output lies over an input");
             }
         }
+        for (const Array &x : out) {
+            for (const Array &y : out) {
+                if (&x < &y && !apart(x, y)) {
+                    throw StatusError(LLAISYS_E_INVALID, "paged plan: two outputs lie over one another");
+                }
+            }
+        }
         if (device_type != LLAISYS_DEVICE_NVIDIA) {
             throw StatusError(LLAISYS_E_UNSUPPORTED, "paged plan: NVIDIA devices only");
         }

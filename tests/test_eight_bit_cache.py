@@ -1126,6 +1126,14 @@ def test_refusals_of_a_plan_whose_arrays_overlap_or_are_not_aligned(changes):
     assert LIB_LLAISYS.llaisysPagedPlanDev(int(llaisys.DeviceType.CPU), 0, ctypes.byref(args), None) == Status.INVALID
 
 
+@pytest.mark.parametrize("changes", [dict(q_starts_dev=1 << 20, kv_lens_dev=1 << 20), dict(q_starts_dev=1 << 20, page_starts_dev=(1 << 20) + 8),
+                                     dict(row_seqs_dev=1 << 20, row_positions_dev=(1 << 20) - 24), dict(status_dev=(1 << 20) + 52, row_slots_dev=1 << 20,
+                                                                                                    block_table_dev=1 << 21, table_rows=4, table_stride=4)])
+def test_refusals_of_a_plan_whose_outputs_lie_over_one_another(changes):
+    args = LlaisysPagedPlan(**(dict(held_dev=4096, new_dev=8192, n_seqs=2, page_size=16, n_rows=7) | changes))
+    assert LIB_LLAISYS.llaisysPagedPlanDev(int(llaisys.DeviceType.CPU), 0, ctypes.byref(args), None) == Status.INVALID
+
+
 def test_arrays_of_a_plan_may_lie_side_by_side():
     args = LlaisysPagedPlan(held_dev=4096, new_dev=4104, n_seqs=2, page_size=16, n_rows=7, kv_lens_dev=4112, q_starts_dev=4084, status_dev=4120)
     assert LIB_LLAISYS.llaisysPagedPlanDev(int(llaisys.DeviceType.CPU), 0, ctypes.byref(args), None) == Status.UNSUPPORTED
