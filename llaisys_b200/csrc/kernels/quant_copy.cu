@@ -8,8 +8,9 @@
 // run to shared memory between the maximum and the rounding (asynchronously, while its place is looked up), so that rows are read once, and stores
 // codes 16 bytes a lane in the order of the tile (quant_tile.cuh): a lane of K takes the four neighbours that make a word of its own; one of V takes
 // four tokens of four dims, turns its 4 x 4 codes round and passes them on through shared memory.
-// Measured: 65536 rows of 2 heads of 128 in bf16, integers, in and back out 42 us (101 MB each way: 4.8 TB/s, bound by issue: a number costs its
-// maximum, a product, a rounding and its share of the byte moves); 64 rows of 64 sequences 7.5 us for both. (Rows held in registers over both passes of
+// Measured: 65536 rows of 2 heads of 128 in bf16, integers, in 21.9 us and back out 20.1 (101 MB each way: 4.6 and 5.0 TB/s; the append
+// issues in 68 % of the cycles -- a number costs its maximum, a product, a rounding and its share of the byte moves -- and waits for its copies a third of a
+// warp's time); 64 rows of 64 sequences 4.0 and 3.5 us. (Rows held in registers over both passes of
 // an append 55 us with the way back, through shared memory with scalar arithmetic 37 + 21.)
 #include "kernels.hpp"
 #include "launch_utils.cuh"
