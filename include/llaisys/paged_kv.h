@@ -277,7 +277,7 @@ LLAISYS_API int llaisysPagedAttentionPrefillDev(llaisysPagedKV_t kv, size_t laye
  * others. A request may appear once. Growth is for callers that keep pages and table themselves: a cache's block manager knows nothing of pages
  * that a plan takes, and gives pages and entries of its own.
  * What cannot be done is left out and flagged, never written elsewhere: rows behind n_rows count as not brought, in every array (the requests they
- * belong to may bring them in a later step); too few free pages take none at all; negative counts and sums over 2^31 - 1 count as nothing brought; a
+ * belong to may bring them in a later step; n_rows 0 with all three row arrays NULL is no limit); too few free pages take none at all; negative counts and sums over 2^31 - 1 count as nothing brought; a
  * request whose row or last page lies outside the table gets no page. Rows that have no page for these reasons are -1 in all three arrays, so that
  * an append skips them too; q_starts and kv_lens count them all the same, and what attention makes of such a request is of no use: the entries behind
  * its pages are not its own. */

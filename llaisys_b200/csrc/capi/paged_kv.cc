@@ -175,7 +175,8 @@ int llaisysPagedPlanDev(llaisysDeviceType_t device_type, int device_id, const Ll
         p.fresh = a->new_dev;
         p.n_seqs = int32_t(a->n_seqs);
         p.page_size = int32_t(a->page_size);
-        p.n_rows = int32_t(a->n_rows);
+        const bool rows_wanted = a->row_seqs_dev != nullptr || a->row_positions_dev != nullptr || a->row_slots_dev != nullptr;
+        p.n_rows = a->n_rows != 0 || rows_wanted ? int32_t(a->n_rows) : int32_t(kMost);
         p.free_pages = a->free_pages_dev;
         p.n_free = a->free_pages_dev ? int32_t(a->n_free) : 0;
         p.table = a->block_table_dev;

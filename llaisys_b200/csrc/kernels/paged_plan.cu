@@ -295,9 +295,10 @@ void paged_plan(stream_t stream, const PlanArgs &args) {
         p.page_shift = p.page_size == 1 << s ? s : p.page_shift;
     }
     p.rows_wide = aligned16(p.row_seqs) && aligned16(p.row_positions) && aligned16(p.row_slots);
+    const bool rows_wanted = p.row_seqs != nullptr || p.row_positions != nullptr || p.row_slots != nullptr;
     // Up to 512 requests, four a thread, small CTAs: their sums take two barriers of four warps instead of 32. A turn of a CTA is four rows a thread.
     auto start = [&](auto kernel, int threads) {
-        const int64_t turns = (std::max<int64_t>(p.n_rows, p.n_seqs) + threads * kRowsAtOnce - 1) / (threads * kRowsAtOnce);
+        const int64_t turns = (std::max<int64_t>(rows_wanted ? p.n_rows : 0, p.n_seqs) + threads * kRowsAtOnce - 1) / (threads * kRowsAtOnce);
         const int64_t most = int64_t(device_sms()) * (threads == 1024 ? 2 : 4);
         kernel<<<unsigned(std::max<int64_t>(1, std::min(turns, most))), threads, 0, static_cast<cudaStream_t>(stream)>>>(p);
     };

@@ -812,7 +812,7 @@ def test_plan_rows_without_a_page_are_not_appended(cuda_device, free, new, flags
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("n,high,long,page", [(3, 40, 30, 16), (64, 300, 9, 16), (700, 100, 20, 48), (2500, 50, 60, 32)])
-@pytest.mark.parametrize("room", [0, 1, 0.37, 0.98])
+@pytest.mark.parametrize("room", [1, 0.37, 0.98])
 def test_plan_of_more_rows_than_there_is_room_for(cuda_device, n, high, long, page, room):
     """Dropped rows are rows that were not brought: lengths, pages and growth agree with the rows that are left."""
     rng = np.random.default_rng(n)
@@ -830,6 +830,24 @@ def test_plan_of_more_rows_than_there_is_room_for(cuda_device, n, high, long, pa
     for key, value in want.items():
         assert np.array_equal(got[key], value), key
     assert np.array_equal(t, w)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [5, 900])
+def test_plan_without_row_arrays(cuda_device, n):
+    """Nothing said about rows, no limit to them: lengths, starts and growth of the whole step."""
+    rng = np.random.default_rng(n)
+    held, new = rng.integers(0, 100, n), rng.integers(0, 40, n)
+    table = np.full((n, 9), 5, np.int32)
+    free = rng.permutation(int((-(-(held + new) // 16) + -held // 16).sum())).astype(np.int32)
+    got, t = run_plan(range(n), held, new, 16, 0, free, table, skip=("row_seqs", "row_positions", "row_slots"))
+    want, w = plan_reference(range(n), held.tolist(), new.tolist(), 16, int(new.sum()), free, table)
+    for key in ("q_starts", "kv_lens", "page_starts", "status"):
+        assert np.array_equal(got[key], want[key]), key
+    assert np.array_equal(t, w)
+    # room for none
+    got, t = run_plan(range(n), held, new, 16, 1, free, table, skip=("row_positions", "row_slots"))
+    assert got["status"].tolist()[1] == 2 and got["q_starts"][-1] == 1
 
 
 @pytest.mark.gpu
