@@ -91,7 +91,8 @@ LLAISYS_API int llaisysPagedKVDestroy(llaisysPagedKV_t kv);
  * so that a block filled token by token is rounded again only when its scale grows. Tokens of the block behind the rows keep their codes,
  * whatever becomes of the scale: a call that writes tokens again leaves those behind them in the block without a value (the other caches
  * leave them as they were), and so are tokens that were never written. A block that a NaN or an infinity is appended to gets the scale NaN,
- * and attention of every query that sees a token of the block is NaN, until its slot 0 is written again.
+ * and attention of every query that sees a token of the block is NaN, until its slot 0 is written again. Attention counts blocks whose values
+ * are all zero in full beside values of up to 10^8 (a row's sum leaves out tokens whose weight times V scale lies 2^125 below its largest).
  * The block manager, llaisysPagedKVAppend(Dev), Gather(Dev), llaisysPagedAttentionDecode(Dev), ...Prefill(Dev), ...DecodePartial(Dev) and
  * llaisysPagedAttentionOptDev (mixers.h) take such a cache with rows, queries and outputs of `dtype`; every other call returns
  * LLAISYS_E_UNSUPPORTED. The rows that one append call brings to a block must be neighbours in the call, in the order of their
